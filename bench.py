@@ -4,7 +4,8 @@
     python bench.py [--gpus N] [--steps K] [--warmup W] [--config 2] [--impl b200|reference]
 
 One step = forward of the whole EGNN over one batch of synthetic graphs,
-graph-sum MSE loss, backward, gradient all-reduce (N > 1) and an SGD update.
+graph-sum MSE loss, backward, gradient all-reduce (N > 1) and an SGD update
+(--optimizer muon: Muon on the weight matrices; --node-norm: normalised layers).
 Default workload: config 2 (512 molecules, 7 layers, H=128, bf16 GEMM
 inputs, fp32 accumulate).  Multi-GPU runs are graph-batch data parallel with
 weak scaling: every rank steps its own 512-graph batch and the gradients are
@@ -37,6 +38,9 @@ def parse():
     ap.add_argument("--n-graphs", type=int, default=None, help="shrink the batch (profiling runs)")
     ap.add_argument("--n-nodes", type=int, default=None, help="config 5: node count (default 2^20)")
     ap.add_argument("--impl", default="b200", choices=["b200", "reference"])
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "muon"],
+                    help="update of the step: SGD, or Muon on the weight matrices and SGD on the rest")
+    ap.add_argument("--node-norm", action="store_true", help="EGNN(node_norm=True): layer norm after every layer")
     ap.add_argument("--allreduce", default="flat", choices=["layers", "flat"],
                     help="data parallel: one flat all-reduce after the backward (flat, measured equal or "
                          "faster at 2 and 8 GPUs) or per-layer buckets all-reduced as the backward "
@@ -244,7 +248,7 @@ class Problem:
 
     def __init__(self, args, world, rank, dev):
         import torch
-        from pymolecular_b200 import CSR, EGNN, graph_sum_mse, parallel
+        from pymolecular_b200 import CSR, EGNN, Muon, graph_sum_mse, parallel
         from pymolecular_b200.datasets import CONFIGS, make_workload
         self.torch, self.parallel, self.CSR = torch, parallel, CSR
         self.graph_sum_mse = graph_sum_mse
@@ -279,9 +283,13 @@ class Problem:
         self.nodes_rank = int(self.h_host.shape[0])
         torch.manual_seed(0)
         self.model = EGNN(mc.in_node_nf, mc.hidden_nf, mc.out_node_nf, n_layers=mc.n_layers, device=dev,
-                          precision=self.precision)
+                          precision=self.precision, node_norm=args.node_norm)
         self.params = list(self.model.parameters())
-        self.opt = torch.optim.SGD(self.params, lr=1e-4)
+        if args.optimizer == "muon":
+            matrices, rest = Muon.split(self.params)
+            self.opts = [Muon(matrices, lr=1e-4), torch.optim.SGD(rest, lr=1e-4)]
+        else:
+            self.opts = [torch.optim.SGD(self.params, lr=1e-4)]
         self.allreduce = "flat" if self.halo else args.allreduce
         names = [n for n, _ in self.model.named_parameters()]
         self.sync_grads = parallel.GradAllReduce(
@@ -314,7 +322,8 @@ class Problem:
         if self.world > 1:
             self.sync_grads.zero_grad()
         else:
-            self.opt.zero_grad(set_to_none=True)
+            for opt in self.opts:
+                opt.zero_grad(set_to_none=True)
 
     def step(self):
         self.zero_grad()
@@ -322,7 +331,8 @@ class Problem:
         loss = self.loss(ho)
         loss.backward()
         self.sync_grads()
-        self.opt.step()
+        for opt in self.opts:
+            opt.step()
         # detached: a captured step must not keep its autograd graph alive
         # past the capture (later eager steps would then accumulate into
         # nodes that belong to the capture stream)
@@ -349,7 +359,8 @@ class Problem:
         loss = self.loss(ho, d.get("gp"), d["tgt"])
         loss.backward()
         self.sync_grads()
-        self.opt.step()
+        for opt in self.opts:
+            opt.step()
         loss_host.copy_(loss.detach().reshape(1), non_blocking=True)
         return csr
 
@@ -628,7 +639,9 @@ def make_line(args, prob, m, world, clk, cpu, dev):
                    "nodes_per_gpu": prob.nodes_rank, "edges_per_gpu": prob.edges_rank,
                    "layers": mc.n_layers, "hidden": H, "precision": prob.precision,
                    "l2": "flushed between timed steps (252 MB write)",
-                   "parallelism": ("nodepart" if prob.halo else "dp") + str(world), "optimizer": "SGD",
+                   "parallelism": ("nodepart" if prob.halo else "dp") + str(world),
+                   "optimizer": "SGD" if args.optimizer == "sgd" else "Muon on the matrices, SGD on the rest",
+                   **({"node_norm": True} if args.node_norm else {}),
                    "allreduce": ("per-layer buckets, issued as the backward produces them"
                                  if prob.allreduce == "layers" else "one flat all-reduce after the backward")
                    if world > 1 else None,

@@ -311,6 +311,99 @@ EGNN_API int egnn_linear_bwd(int64_t m, int32_t k, int32_t o, const float* x, co
 EGNN_API int egnn_linear_bwd_static(int64_t m, int32_t k, int32_t o, const float* x, const float* w,
                                     const float* dy, float* dx, float* dw, float* db, void* stream);
 
+/* ---- layer normalisation of node features ------------------------------- */
+
+/* Element types of the normalised rows and of the orthogonalised matrices. */
+enum { EGNN_DTYPE_F32 = 0, EGNN_DTYPE_BF16 = 1, EGNN_DTYPE_F16 = 2 };
+
+/* y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis of
+ * x (rows, cols), cols <= 8192, row stride ldx elements; y dense (rows, cols).
+ * x and y have type `dtype`; weight and bias (cols; either may be NULL) have
+ * type param_dtype: float32 or `dtype`.  var is the mean squared distance
+ * from the mean; every sum is float32.  stats (may be NULL in inference)
+ * receives 2 floats per row, the mean and 1 / sqrt(var + eps), for the
+ * backward.  No counterpart in the reference. */
+EGNN_API int egnn_layer_norm_fwd(int64_t rows, int32_t cols, const void* x, int64_t ldx, int32_t dtype,
+                                 const void* weight, const void* bias, int32_t param_dtype, float eps, void* y,
+                                 float* stats, void* stream);
+
+/* Scratch bytes of egnn_layer_norm_bwd (0: shape not built). */
+EGNN_API size_t egnn_layer_norm_workspace_size(int64_t rows, int32_t cols);
+
+/* Backward of egnn_layer_norm_fwd given dy (row stride lddy, type dtype) and
+ * the forward's stats: dx dense (rows, cols) in `dtype`, dweight and dbias
+ * (cols) in param_dtype, all overwritten; each may be NULL to skip it.  The
+ * workspace is used only for dweight and dbias.  Deterministic. */
+EGNN_API int egnn_layer_norm_bwd(int64_t rows, int32_t cols, const void* x, int64_t ldx, const void* dy,
+                                 int64_t lddy, int32_t dtype, const void* weight, int32_t param_dtype,
+                                 const float* stats, void* dx, void* dweight, void* dbias, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* ---- orthogonalised updates (Newton-Schulz) ------------------------------ */
+
+/* The iteration: X0 = G / (|G|_F + eps), transposed where rows > cols, then
+ * `steps` times X <- a X + (b A + c A A) X with A = X X^T.  It acts on the
+ * singular values alone: s <- a s + b s^3 + c s^5.  The coefficients must
+ * keep the singular values that start in [0, 1] below 1024 in every step
+ * (EGNN_ERR_INVALID_ARG otherwise). */
+typedef struct {
+  int32_t steps;     /* 0 .. 64 */
+  int32_t reserved;  /* 0 */
+  double a, b, c;
+  double eps;        /* >= 0 */
+} egnn_ns_options;
+
+/* One matrix of egnn_orthogonalize: in and out (rows, cols) row-major, row
+ * strides ld_in / ld_out elements, both of type dtype; out == in with equal
+ * strides is allowed, any other overlap is not. */
+typedef struct {
+  const void* in;
+  void* out;
+  int64_t ld_in, ld_out;
+  int32_t rows, cols;    /* 0 .. 16384 each, and the smaller at most 1024 */
+  int32_t dtype;
+  int32_t reserved;      /* 0 */
+} egnn_matrix;
+
+/* Scratch bytes of egnn_orthogonalize / egnn_muon_step for matrices of these
+ * sizes (HOST array of `count` (rows, cols) pairs; 0: a size is not built). */
+EGNN_API size_t egnn_orthogonalize_workspace_size(int64_t count, const int32_t* sizes);
+
+/* out_k = the orthogonalised in_k for every matrix of the HOST array `m`
+ * (read before the call returns).  Products are as exact as float32's.
+ * Deterministic.  No counterpart in the reference. */
+EGNN_API int egnn_orthogonalize(int64_t count, const egnn_matrix* m, const egnn_ns_options* o, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* One weight matrix of egnn_muon_step (float32, row-major, row strides in
+ * elements); no two of a call's weights and momenta may overlap. */
+typedef struct {
+  float* weight;
+  const float* grad;
+  float* momentum;
+  int64_t ld_weight, ld_grad, ld_momentum;
+  int32_t rows, cols;    /* as in egnn_matrix */
+  float gain;            /* factor of this matrix's update */
+  int32_t reserved;      /* 0 */
+} egnn_muon_matrix;
+
+typedef struct {
+  egnn_ns_options ns;
+  double momentum;         /* mu in [0, 1) */
+  double weight_decay;
+  double lr;               /* used where lr_device is NULL */
+  const float* lr_device;  /* one device float, read when the kernels run (captured steps) */
+  int32_t nesterov;        /* 0 or 1 */
+  int32_t reserved;        /* 0 */
+} egnn_muon_options;
+
+/* For every matrix: momentum <- mu momentum + (1 - mu) grad;
+ * U = mu momentum + (1 - mu) grad (nesterov) or momentum;
+ * weight <- (1 - lr weight_decay) weight - lr gain orthogonalised(U).
+ * Weights and momenta are updated in place; deterministic. */
+EGNN_API int egnn_muon_step(int64_t count, const egnn_muon_matrix* m, const egnn_muon_options* o, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ---- diagnostics ------------------------------------------------------- */
 
 /* Copies the calling thread's last error message into buf (NUL-terminated);

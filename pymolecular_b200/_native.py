@@ -6,6 +6,7 @@ the shared object is missing or fails to load, every call raises
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -27,6 +28,10 @@ FLAG_ATTENTION = 2
 FLAG_NORMALIZE = 4
 FLAG_TANH = 8
 FLAG_COORDS_SUM = 16
+
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+DTYPE_F16 = 2
 
 PREC_FP32 = 0
 PREC_BF16 = 1
@@ -83,6 +88,27 @@ class LayerGrads(C.Structure):
     _fields_ = [(f, VP) for f in _PARAM_FIELDS]
 
 
+class NsOptions(C.Structure):
+    _fields_ = [("steps", C.c_int32), ("reserved", C.c_int32), ("a", C.c_double), ("b", C.c_double), ("c", C.c_double),
+                ("eps", C.c_double)]
+
+
+class Matrix(C.Structure):
+    _fields_ = [("in_", VP), ("out", VP), ("ld_in", C.c_int64), ("ld_out", C.c_int64), ("rows", C.c_int32),
+                ("cols", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class MuonMatrix(C.Structure):
+    _fields_ = [("weight", VP), ("grad", VP), ("momentum", VP), ("ld_weight", C.c_int64), ("ld_grad", C.c_int64),
+                ("ld_momentum", C.c_int64), ("rows", C.c_int32), ("cols", C.c_int32), ("gain", C.c_float),
+                ("reserved", C.c_int32)]
+
+
+class MuonOptions(C.Structure):
+    _fields_ = [("ns", NsOptions), ("momentum", C.c_double), ("weight_decay", C.c_double), ("lr", C.c_double),
+                ("lr_device", VP), ("nesterov", C.c_int32), ("reserved", C.c_int32)]
+
+
 # name -> (restype, argtypes)
 _SIGNATURES = {
     "egnn_csr_workspace_size": (C.c_size_t, [C.c_int64, C.c_int64]),
@@ -113,6 +139,14 @@ _SIGNATURES = {
     "egnn_linear_bwd": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, VP, VP, VP, VP, VP, VP, VP,
                                   C.c_size_t, VP]),
     "egnn_linear_bwd_static": (C.c_int, [C.c_int64, C.c_int32, C.c_int32, VP, VP, VP, VP, VP, VP, VP]),
+    "egnn_layer_norm_fwd": (C.c_int, [C.c_int64, C.c_int32, VP, C.c_int64, C.c_int32, VP, VP, C.c_int32, C.c_float,
+                                      VP, VP, VP]),
+    "egnn_layer_norm_workspace_size": (C.c_size_t, [C.c_int64, C.c_int32]),
+    "egnn_layer_norm_bwd": (C.c_int, [C.c_int64, C.c_int32, VP, C.c_int64, VP, C.c_int64, C.c_int32, VP, C.c_int32,
+                                      VP, VP, VP, VP, VP, C.c_size_t, VP]),
+    "egnn_orthogonalize_workspace_size": (C.c_size_t, [C.c_int64, VP]),
+    "egnn_orthogonalize": (C.c_int, [C.c_int64, VP, C.POINTER(NsOptions), VP, C.c_size_t, VP]),
+    "egnn_muon_step": (C.c_int, [C.c_int64, VP, C.POINTER(MuonOptions), VP, C.c_size_t, VP]),
     "egnn_last_error": (C.c_size_t, [C.c_char_p, C.c_size_t]),
     "egnn_version": (C.c_char_p, []),
     "egnn_device_status": (C.c_int, [VP]),
@@ -178,3 +212,12 @@ def stream_ptr(stream=None) -> int:
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
+
+
+def device_of(t):
+    """Context in which `t`'s device is the current one."""
+    import torch
+    return _SAME if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_SAME = contextlib.nullcontext()

@@ -17,7 +17,11 @@ signatures as the reference ``models/EGNN/egnn_clean.py``:
 reference's ``[row, col]`` pair (converted once, on the GPU, by a stable sort).
 Parameters keep the reference ``state_dict`` names, so checkpoints move both
 ways.  One extra keyword, ``precision='fp32' | 'bf16'``, selects fp32 GEMMs
-(default) or bf16 GEMM inputs with fp32 accumulation.
+(default) or bf16 GEMM inputs with fp32 accumulation; another,
+``EGNN(..., node_norm=True)``, normalises the node features after every layer
+(``norm_%d``, an ``nn.LayerNorm(hidden_nf)`` run by ``norm.layer_norm``),
+which the reference does not have: without it (the default) the parameters
+and results are the reference's.
 
 ``E_GCL`` takes any ``input_nf`` / ``output_nf`` next to ``hidden_nf`` (as
 the reference constructor does; ``EGNN`` builds every layer with all three
@@ -39,6 +43,7 @@ from torch import nn
 
 from . import _native as nat
 from .csr import CSR, as_csr
+from .norm import layer_norm
 
 _PARAM_ORDER = ["edge_mlp.0.weight", "edge_mlp.0.bias", "edge_mlp.2.weight", "edge_mlp.2.bias",
                 "node_mlp.0.weight", "node_mlp.0.bias", "node_mlp.2.weight", "node_mlp.2.bias",
@@ -247,10 +252,11 @@ class EGNN(nn.Module):
 
     def __init__(self, in_node_nf, hidden_nf, out_node_nf, in_edge_nf=0, device='cpu',
                  act_fn=nn.SiLU(), n_layers=4, residual=True, attention=False, normalize=False,
-                 tanh=False, precision: str = "fp32"):
+                 tanh=False, precision: str = "fp32", node_norm: bool = False):
         super().__init__()
         self.hidden_nf = hidden_nf
         self.device = device
+        self.node_norm = node_norm
         self.n_layers = n_layers
         self.embedding_in = nn.Linear(in_node_nf, self.hidden_nf)
         self.embedding_out = nn.Linear(self.hidden_nf, out_node_nf)
@@ -260,6 +266,8 @@ class EGNN(nn.Module):
                                                 residual=residual, attention=attention,
                                                 normalize=normalize, tanh=tanh,
                                                 precision=precision))
+            if node_norm:   # draws nothing: the other parameters keep their seeded values
+                self.add_module("norm_%d" % i, nn.LayerNorm(self.hidden_nf))
         self.to(self.device)
 
     @property
@@ -271,12 +279,17 @@ class EGNN(nn.Module):
         for i in range(self.n_layers):
             self._modules["gcl_%d" % i].precision = value
 
+    def normalized(self, i, h):
+        """h after layer i: normalised with norm_i where the model has norms."""
+        return layer_norm(h, self._modules["norm_%d" % i]) if self.node_norm else h
+
     def forward(self, h, x, edges, edge_attr=None):
         h = _check_tensor(h, "h")
         csr = as_csr(edges, h.shape[0], h.device)
         h = linear(h, self.embedding_in)
         for i in range(0, self.n_layers):
             h, x, _ = self._modules["gcl_%d" % i](h, csr, x, edge_attr=edge_attr)
+            h = self.normalized(i, h)
         h = linear(h, self.embedding_out)
         return h, x
 

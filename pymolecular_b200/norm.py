@@ -1,0 +1,107 @@
+"""Layer normalisation of node features on the library's kernels.
+
+``layer_norm(x, layer)`` is the forward of an ``nn.LayerNorm`` over the last
+axis, ``(x - mean) / sqrt(var + eps) * weight + bias``, with its backward
+(dx, and the weight's and bias's gradients summed over all rows in a fixed
+order) in ``egnn_layer_norm_fwd`` / ``egnn_layer_norm_bwd``.  It stands next
+to ``linear`` (``nn.Linear`` on the library's node GEMM); ``EGNN`` calls it
+between its layers when built with ``node_norm=True``.
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import _native as nat
+
+DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
+
+
+def _forward(x, weight, bias, eps, stats):
+    """y and, where asked for, the (rows, 2) mean and 1 / sqrt(var + eps)."""
+    rows, cols = x.shape
+    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    kept = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if stats else None
+    p = weight if weight is not None else bias
+    with nat.device_of(x):
+        nat.check(nat.lib().egnn_layer_norm_fwd(rows, cols, nat.ptr(x), x.stride(0), DTYPES[x.dtype], nat.ptr(weight),
+                                                nat.ptr(bias), nat.DTYPE_F32 if p is None else DTYPES[p.dtype], eps,
+                                                nat.ptr(y), nat.ptr(kept), nat.stream_ptr()), "egnn_layer_norm_fwd")
+    return y, kept
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        rows, cols = x.shape
+        dy = _rows(dy)
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        pdt = weight.dtype if weight is not None else ctx.bias_dtype or torch.float32
+        dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty(cols, dtype=pdt, device=x.device) if need_w else None
+        db = torch.empty(cols, dtype=pdt, device=x.device) if need_b else None
+        lib = nat.lib()
+        with nat.device_of(x):
+            ws, ws_bytes = None, 0
+            if need_w or need_b:
+                ws_bytes = lib.egnn_layer_norm_workspace_size(rows, cols)
+                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+            nat.check(lib.egnn_layer_norm_bwd(rows, cols, nat.ptr(x), x.stride(0), nat.ptr(dy), dy.stride(0),
+                                              DTYPES[x.dtype], nat.ptr(weight), DTYPES[pdt], nat.ptr(stats),
+                                              nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.ptr(ws), ws_bytes,
+                                              nat.stream_ptr()), "egnn_layer_norm_bwd")
+        return dx, dw, db, None
+
+
+def _rows(t):
+    """t itself where its rows are dense and do not overlap, else a copy."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def layer_norm(x: torch.Tensor, layer: nn.LayerNorm) -> torch.Tensor:
+    """nn.LayerNorm forward (over the last axis) on the library's kernels.
+
+    x: (..., C) float32, bfloat16 or float16 CUDA, C <= 8192; rows may be a
+    slice of wider ones.  The layer's weight and bias (either may be absent)
+    are float32 or of x's type, both of one type.  The result has x's type;
+    statistics and sums are float32.
+    """
+    if not x.is_cuda:
+        raise ValueError("layer_norm takes CUDA tensors (pymolecular_b200 has no CPU path)")
+    if x.dtype not in DTYPES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    shape = layer.normalized_shape
+    if len(shape) != 1 or x.dim() < 1 or x.shape[-1] != shape[0]:
+        raise ValueError(f"x must be (..., C) for a LayerNorm over its last axis alone, got {tuple(x.shape)} and "
+                         f"normalized_shape {tuple(shape)}")
+    weight, bias = layer.weight, layer.bias
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.device != x.device:
+            raise ValueError(f"the layer's {name} must be on {x.device}, got {p.device}")
+        if p.dtype not in (torch.float32, x.dtype) or (weight is not None and p.dtype != weight.dtype):
+            raise TypeError(f"the layer's {name} must be float32 or {x.dtype}, both parameters of one type, got {p.dtype}")
+    rows = x if x.dim() == 2 else x.reshape(-1, shape[0])
+    if rows.shape[0] > 1 or rows.stride(1) != 1:
+        rows = _rows(rows)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        y = _LayerNormFn.apply(rows, weight, bias, layer.eps)
+    else:
+        y, _ = _forward(rows, weight, bias, layer.eps, False)
+    return y if x.dim() == 2 else y.view(x.shape)
+
+
+__all__ = ["layer_norm"]

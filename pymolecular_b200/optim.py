@@ -1,0 +1,197 @@
+"""The update of a model's weight matrices: momentum, orthogonalised by
+Newton-Schulz products (the Muon optimiser), on the library's kernels.
+
+* ``orthogonalize(g)``: X0 = G / (|G|_F + eps), then ``steps`` times
+  X <- a X + (b A + c A A) X with A = X X^T, which moves the singular values
+  by s <- a s + b s^3 + c s^5 and keeps the singular vectors.  One matrix, a
+  batch, or a list of matrices of any sizes in one call
+  (``egnn_orthogonalize``).
+* ``muon_step(params, grads, buffers, lr)``: for every matrix
+  M <- mu M + (1 - mu) G, U = mu M + (1 - mu) G (Nesterov) or M,
+  W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(U)
+  (``egnn_muon_step``), in place.
+* ``Muon``: the same as a ``torch.optim.Optimizer`` for an ``EGNN``'s weight
+  matrices (``Muon.split`` separates them from its vectors).
+
+All matrices of a call share its launches; nothing synchronises with the
+host, so a step with them can be captured (``graphs.GraphedStep``).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Iterable, List, Sequence, Tuple, Union
+
+import torch
+
+from . import _native as nat
+from .norm import DTYPES
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+STEPS = 5
+EPS = 1e-7
+
+
+def _options(steps, coefficients, eps):
+    a, b, c = coefficients
+    return nat.NsOptions(int(steps), 0, a, b, c, eps)
+
+
+def _workspace(sizes: Sequence[int], device) -> Tuple[torch.Tensor, int]:
+    count = len(sizes) // 2
+    nbytes = nat.lib().egnn_orthogonalize_workspace_size(count, (C.c_int32 * len(sizes))(*sizes))
+    if not nbytes:
+        raise ValueError("matrices have at most 16384 rows and columns, and the smaller side at most 1024")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+
+
+def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = STEPS,
+                  coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = EPS):
+    """The matrix, batch of matrices (..., m, n) or list of matrices `g` with
+    its singular values driven towards 1 by `steps` Newton-Schulz products.
+
+    float32, bfloat16 or float16 CUDA tensors of one device; the result has
+    each one's type and shape (dense), the products are as exact as
+    float32's.  Not differentiable: it treats `g` as data.
+    """
+    if isinstance(g, torch.Tensor):
+        if g.dim() < 2:
+            raise ValueError("orthogonalize takes matrices")
+        if g.dim() == 2:
+            return orthogonalize([g], steps, coefficients, eps)[0]
+        flat = g.detach().reshape(-1, *g.shape[-2:])
+        out = torch.empty(flat.shape, dtype=g.dtype, device=g.device)
+        _orthogonalize(list(flat), list(out), steps, coefficients, eps)
+        return out.view(g.shape)
+    mats = [t.detach() for t in g]
+    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in mats]
+    _orthogonalize(mats, out, steps, coefficients, eps)
+    return out
+
+
+def _orthogonalize(mats, out, steps, coefficients, eps):
+    if not mats:
+        return
+    device = mats[0].device
+    sizes, items = [], (nat.Matrix * len(mats))()
+    keep = []
+    for k, (t, o) in enumerate(zip(mats, out)):
+        if not t.is_cuda:
+            raise ValueError("orthogonalize takes CUDA tensors (pymolecular_b200 has no CPU path)")
+        if t.device != device:
+            raise ValueError("the matrices of a call must be on one device")
+        if t.dtype not in DTYPES:
+            raise TypeError(f"matrices must be float32, bfloat16 or float16, got {t.dtype}")
+        if t.dim() != 2:
+            raise ValueError("orthogonalize takes matrices")
+        t = t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+        keep.append(t)
+        rows, cols = t.shape
+        sizes += [rows, cols]
+        items[k] = nat.Matrix(nat.ptr(t), nat.ptr(o), t.stride(0), cols, rows, cols, DTYPES[t.dtype], 0)
+    with nat.device_of(mats[0]):
+        ws, nbytes = _workspace(sizes, device)
+        nat.check(nat.lib().egnn_orthogonalize(len(mats), items, C.byref(_options(steps, coefficients, eps)),
+                                               nat.ptr(ws), nbytes, nat.stream_ptr()), "egnn_orthogonalize")
+
+
+def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buffers: Sequence[torch.Tensor],
+              lr: Union[float, torch.Tensor], momentum: float = 0.95, nesterov: bool = True,
+              weight_decay: float = 0.0, steps: int = STEPS,
+              coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = EPS) -> None:
+    """One momentum step with orthogonalised updates, in place on `params` and
+    their momenta `buffers` (float32 CUDA matrices with dense rows, no two of
+    them overlapping).  `lr` is a number or a one-element float32 CUDA tensor,
+    which a captured step reads at each replay."""
+    params, grads, buffers = list(params), list(grads), list(buffers)
+    if not len(params) == len(grads) == len(buffers):
+        raise ValueError("muon_step takes one gradient and one momentum buffer for each parameter")
+    if not params:
+        return
+    if len({t.data_ptr() for t in (*params, *buffers) if t.numel()}) < sum(t.numel() > 0 for t in (*params, *buffers)):
+        raise ValueError("a parameter or momentum buffer is given twice")
+    device = params[0].device
+    on_device = isinstance(lr, torch.Tensor)
+    if on_device and (lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != device):
+        raise ValueError("lr must be a number or one float32 on the parameters' device")
+    sizes, items, keep = [], (nat.MuonMatrix * len(params))(), []
+    for k, (p, g, m) in enumerate(zip(params, grads, buffers)):
+        if not p.is_cuda:
+            raise ValueError("muon_step takes CUDA tensors (pymolecular_b200 has no CPU path)")
+        if p.dim() != 2 or p.shape != g.shape or p.shape != m.shape:
+            raise ValueError(f"parameter {k}: a matrix and its gradient and momentum of the same shape are needed, got "
+                             f"{tuple(p.shape)}, {tuple(g.shape)}, {tuple(m.shape)}")
+        if p.device != device or g.device != device or m.device != device:
+            raise ValueError("the tensors of a step must be on one device")
+        if p.dtype != torch.float32 or g.dtype != torch.float32 or m.dtype != torch.float32:
+            raise TypeError("muon_step takes float32 parameters, gradients and momenta")
+        rows, cols = p.shape
+        for t in (p, m):
+            if rows * cols and (t.stride(1) != 1 and cols > 1 or t.stride(0) < cols and rows > 1):
+                raise ValueError("parameters and momenta must have dense rows (they are updated in place)")
+        g = g if g.stride(1) == 1 and g.stride(0) >= cols else g.contiguous()
+        keep.append(g)
+        sizes += [rows, cols]
+        items[k] = nat.MuonMatrix(nat.ptr(p), nat.ptr(g), nat.ptr(m), p.stride(0), g.stride(0), m.stride(0), rows, cols,
+                                  max(1.0, rows / max(cols, 1)) ** 0.5, 0)
+    options = nat.MuonOptions(_options(steps, coefficients, eps), momentum, weight_decay,
+                              0.0 if on_device else lr, nat.ptr(lr) if on_device else None, int(nesterov), 0)
+    with nat.device_of(params[0]):
+        ws, nbytes = _workspace(sizes, device)
+        nat.check(nat.lib().egnn_muon_step(len(params), items, C.byref(options), nat.ptr(ws), nbytes, nat.stream_ptr()),
+                  "egnn_muon_step")
+    torch.autograd.graph.increment_version((*params, *buffers))
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum with orthogonalised updates for weight matrices.
+
+    Takes float32 matrices only: an ``EGNN``'s weights go here, its biases and
+    normalisation vectors to another optimiser (``Muon.split``).  `lr` may be
+    a one-element CUDA tensor (captured steps).  State: ``momentum_buffer``.
+    """
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 0.02, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = STEPS,
+                 coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = EPS):
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"lr must not be negative, got {lr}")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"momentum must be in [0, 1), got {momentum}")
+        if not weight_decay >= 0.0:
+            raise ValueError(f"weight_decay must not be negative, got {weight_decay}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      steps=steps, coefficients=tuple(coefficients), eps=eps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() != 2 or p.dtype != torch.float32:
+                    raise ValueError(f"Muon takes float32 matrices, got {tuple(p.shape)} {p.dtype} (Muon.split gives "
+                                     "them and the rest apart)")
+
+    @staticmethod
+    def split(params: Iterable[torch.Tensor]) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
+        """(matrices with more than one row and column, the rest)."""
+        params = list(params)
+        mats = [p for p in params if p.dim() == 2 and min(p.shape) > 1]
+        chosen = {id(p) for p in mats}
+        return mats, [p for p in params if id(p) not in chosen]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            params = [p for p in group["params"] if p.grad is not None]
+            buffers = []
+            for p in params:
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                buffers.append(state["momentum_buffer"])
+            muon_step(params, [p.grad for p in params], buffers, group["lr"], group["momentum"], group["nesterov"],
+                      group["weight_decay"], group["steps"], group["coefficients"], group["eps"])
+        return loss
+
+
+__all__ = ["COEFFICIENTS", "Muon", "muon_step", "orthogonalize"]

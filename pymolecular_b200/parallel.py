@@ -347,7 +347,8 @@ def partitioned_forward(model, h_own: torch.Tensor, x_own: torch.Tensor, csr_loc
 
     embedding_in on the owned rows; before every layer the halo rows of h
     and x are fetched; each layer runs on the local graph (owned rows plus
-    halo rows, edges into owned rows only) and keeps its owned rows;
+    halo rows, edges into owned rows only) and keeps its owned rows
+    (normalised where the model has norms);
     embedding_out on the owned rows.  In bf16-GEMM mode the halo rows of h
     travel as bf16 (the coordinates and all gradients stay fp32).  Returns
     (h_out_own, x_out_own)."""
@@ -360,7 +361,7 @@ def partitioned_forward(model, h_own: torch.Tensor, x_own: torch.Tensor, csr_loc
         h_loc = halo_exchange(h, plan, group, wire_dtype=wire)
         x_loc = halo_exchange(x, plan, group)
         h_loc, x_loc, _ = model._modules["gcl_%d" % i](h_loc, csr_local, x_loc)
-        h, x = h_loc[:n_own], x_loc[:n_own]
+        h, x = model.normalized(i, h_loc[:n_own]), x_loc[:n_own]
     return linear(h.contiguous(), model.embedding_out), x
 
 
