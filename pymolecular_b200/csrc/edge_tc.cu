@@ -36,6 +36,7 @@
 #include "edge_rows.cuh"
 #include "edge_simt.cuh"
 #include "edge_tc.cuh"
+#include "newton_schulz.cuh"
 #include "node_tc.cuh"
 #include "tc.cuh"
 
@@ -1335,6 +1336,7 @@ extern "C" int egnn_device_status(void* stream) {
   }
   n += node_tc_take_timeouts();
   n += rows_take_timeouts();
+  n += ns_fused_take_timeouts();
   if (n != 0) {
     return fail(EGNN_ERR_CUDA, "%d tensor-core wait(s) timed out; results are invalid", n);
   }

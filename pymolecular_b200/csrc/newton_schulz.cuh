@@ -1,0 +1,75 @@
+// Shared between the Newton-Schulz kernels: descriptors of the matrices of a
+// launch, the scalars of a call, element access.
+#pragma once
+
+#include <algorithm>
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace egnn {
+
+constexpr int kNsItems = 64;   // matrices of one launch (kernel parameters)
+
+struct NsItem {
+  const void* in;        // the matrix, or the gradient (float32) of a step
+  void* out;             // its orthogonalised form, or the weight of a step
+  float* mom;            // momentum of a step; NULL: no step
+  int64_t ld_in, ld_out, ld_mom;
+  int rows, cols, dtype;
+  float gain;
+};
+
+struct NsBatch {
+  NsItem it[kNsItems];
+  int count;
+};
+
+// X, A and B = b A + c A A are kept as fp16 pairs hi + lo (22 bits) scaled by
+// powers of two, chosen so that their largest entries stay near 2^14: the
+// iteration bounds the singular values, hence every entry, beforehand.
+struct NsScalars {
+  float a, b, c;
+  double eps;
+  float sx, sa, sb;         // scales of X, A and B
+  float mu, nu;             // nu = 1 - mu
+  double decay, lr;
+  const float* lr_device;
+  int nesterov;
+  int steps;
+};
+
+__device__ __forceinline__ float ns_load(const void* p, int dtype, int64_t i) {
+  if (dtype == EGNN_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == EGNN_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void ns_store(void* p, int dtype, int64_t i, float v) {
+  if (dtype == EGNN_DTYPE_F32) static_cast<float*>(p)[i] = v;
+  else if (dtype == EGNN_DTYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// M <- mu M + nu G, and U = mu M + nu G (Nesterov) or M from the moved M.
+__device__ __forceinline__ float ns_momentum(const NsScalars& q, float g, float m) { return fmaf(q.mu, m, q.nu * g); }
+__device__ __forceinline__ float ns_update(const NsScalars& q, float g, float m) {
+  return q.nesterov ? fmaf(q.mu, m, q.nu * g) : m;
+}
+
+// Factors of W <- keep W + move O.
+__device__ __forceinline__ void ns_rates(const NsItem& it, const NsScalars& q, float& keep, float& move) {
+  const double lr = q.lr_device ? (double)*q.lr_device : q.lr;
+  keep = (float)(1.0 - lr * q.decay);
+  move = (float)(-lr * it.gain);
+}
+
+// Whether one block's shared memory holds the whole iteration of an m x n
+// matrix (m <= n).
+bool ns_fused_fits(int m, int n);
+// The matrices of the batch, one block each.
+int ns_fused(const NsBatch& b, const NsScalars& q, cudaStream_t s);
+// Waits that ran out since the last call.
+int ns_fused_take_timeouts();
+
+}  // namespace egnn
