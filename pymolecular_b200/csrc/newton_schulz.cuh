@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_fp16.h>
 
@@ -40,6 +41,15 @@ struct NsScalars {
   int steps;
 };
 
+__device__ __forceinline__ float ns_float(float v) { return v; }
+__device__ __forceinline__ float ns_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float ns_float(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T ns_from(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
 __device__ __forceinline__ float ns_load(const void* p, int dtype, int64_t i) {
   if (dtype == EGNN_DTYPE_F32) return static_cast<const float*>(p)[i];
   if (dtype == EGNN_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);

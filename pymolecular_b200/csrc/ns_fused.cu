@@ -79,45 +79,225 @@ __device__ __forceinline__ void load_pairs32(const char* hi, const char* lo, int
   }
 }
 
-__device__ __forceinline__ uint64_t desc_k(const char* tile, int R, int kk) {
-  return make_desc(smem_u32(tile) + (kk >> 2) * R * 128 + (kk & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t desc_mn(const char* tile, int R, int c0, int kk) {
-  return make_desc(smem_u32(tile) + (c0 >> 6) * R * 128 + kk * 2048, R * 128, 1024);
-}
-
-constexpr int kBatch = 8;
-
-// The elements tid, tid + kThreads, ... of a matrix, kBatch at a time.
-struct Walk {
-  int r[kBatch];
-  int c[kBatch];
-  int rows, cols, dr, dc;
-  __device__ __forceinline__ Walk(const NsItem& it, int tid)
-      : rows(it.rows), cols(it.cols), dr(kThreads / it.cols), dc(kThreads % it.cols) {
-    r[0] = tid / it.cols;
-    c[0] = tid % it.cols;
-    spread();
+// The same places hold a float32's upper and lower 16 bits before the first
+// product and after the last.
+__device__ __forceinline__ void store_raw32(char* hi, char* lo, int R, int row, int c0, const float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t x = __float_as_uint(v[8 * j + 2 * k]), y = __float_as_uint(v[8 * j + 2 * k + 1]);
+      h[k] = __byte_perm(x, y, 0x7632);
+      l[k] = __byte_perm(x, y, 0x5410);
+    }
+    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
+    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
   }
-  __device__ __forceinline__ void step(int to, int from) {
-    r[to] = r[from] + dr;
-    c[to] = c[from] + dc;
-    if (c[to] >= cols) {
-      c[to] -= cols;
-      ++r[to];
+}
+__device__ __forceinline__ void load_raw32(const char* hi, const char* lo, int R, int row, int c0, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
+    const uint4 h = *reinterpret_cast<const uint4*>(hi + at), l = *reinterpret_cast<const uint4*>(lo + at);
+    const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[8 * j + 2 * k] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x5410));
+      v[8 * j + 2 * k + 1] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x7632));
     }
   }
-  __device__ __forceinline__ void spread() {
+}
+
+// Issues D (+)= L R over nk K-steps of 16.  L is K-major; R is K-major, or
+// MN-major from column c0 on.  Tiles of `rows` rows; only the address field of
+// the descriptors moves.
+template <bool MN>
+__device__ __forceinline__ void issue(uint32_t one, uint32_t d, const char* L, const char* Rt, int rows, int c0, int nk, uint32_t idesc,
+                                      bool accumulate) {
+  const uint32_t blk = rows * 128;
+  uint64_t l = make_desc(smem_u32(L), 16, 1024);
+  uint64_t r = MN ? make_desc(smem_u32(Rt) + (c0 >> 6) * blk, blk, 1024) : make_desc(smem_u32(Rt), 16, 1024);
+  uint32_t acc = accumulate;
+#pragma unroll 1
+  for (int k0 = 0; k0 < nk; k0 += 4) {
 #pragma unroll
-    for (int k = 1; k < kBatch; ++k) step(k, k - 1);
+    for (int j = 0; j < 4; ++j)
+      if (k0 + j < nk) {
+        mma_f16_elected(one, d, l + 2 * j, r + (MN ? 128 : 2) * j, idesc, acc);
+        acc = 1;
+      }
+    l += blk >> 4;
+    r += MN ? 512 : blk >> 4;
   }
-  __device__ __forceinline__ bool any() const { return r[0] < rows; }
-  __device__ __forceinline__ bool has(int k) const { return r[k] < rows; }
+}
+// lo hi + hi lo + hi hi, in this order.
+template <bool MN>
+__device__ __forceinline__ void issue3(uint32_t one, uint32_t d, const char* Lh, const char* Ll, const char* Rh, const char* Rl, int rows,
+                                       int c0, int nk, uint32_t idesc) {
+  issue<MN>(one, d, Ll, Rh, rows, c0, nk, idesc, false);
+  issue<MN>(one, d, Lh, Rl, rows, c0, nk, idesc, true);
+  issue<MN>(one, d, Lh, Rh, rows, c0, nk, idesc, true);
+}
+
+// A warp's share of a matrix in global memory: units of 8 rows x 32 columns,
+// a column to a lane, so that an element costs few instructions besides its
+// access: the swizzle of row k of a unit is a constant of k.  In a turned
+// matrix the 8 rows are one 16-byte chunk of a tile row.
+struct Unit {
+  int id, per_row, r0, c;
+  __device__ __forceinline__ Unit(int cols) : id(threadIdx.x >> 5), per_row((cols + 31) >> 5) { place(); }
+  __device__ __forceinline__ void place() {
+    r0 = id / per_row * 8;
+    c = id % per_row * 32 + (threadIdx.x & 31);
+  }
   __device__ __forceinline__ void next() {
-    step(0, kBatch - 1);
-    spread();
+    id += kWarps;
+    place();
   }
 };
+// Tile offset of element (r0 + k, c): chunk (k, in the low bits) of a tile whose column blocks are blk bytes.
+__device__ __forceinline__ uint32_t unit_row(const Unit& u, uint32_t blk, int k) {
+  return (u.c >> 6) * blk + ((u.r0 + k) << 7) + ((((u.c >> 3) & 7) ^ k) << 4) + ((u.c & 7) << 1);
+}
+__device__ __forceinline__ uint32_t unit_chunk(const Unit& u, uint32_t blk) {
+  return (u.r0 >> 6) * blk + (u.c << 7) + ((((u.r0 >> 3) & 7) ^ (u.c & 7)) << 4);
+}
+
+// The unit's 8 elements of this lane; zeros outside the matrix.
+template <typename T>
+__device__ __forceinline__ void unit_load(const T* p, int64_t ld, const Unit& u, int rows, int cols, float (&v)[8]) {
+  const int n = u.c < cols ? rows - u.r0 : 0;
+  p += u.r0 * ld + u.c;
+#pragma unroll
+  for (int k = 0; k < 8; ++k, p += ld) v[k] = k < n ? ns_float(*p) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void unit_store(T* p, int64_t ld, const Unit& u, int rows, int cols, const float (&v)[8]) {
+  const int n = u.c < cols ? rows - u.r0 : 0;
+  p += u.r0 * ld + u.c;
+#pragma unroll
+  for (int k = 0; k < 8; ++k, p += ld)
+    if (k < n) *p = ns_from<T>(v[k]);
+}
+
+// U into the tiles (raw); returns this thread's sum of squares, added in
+// float64: no overflow or underflow at any scale of the gradient.  The next
+// unit's loads are in flight while a unit is worked on.
+template <typename T, bool MOM>
+__device__ __forceinline__ double take_in(const NsItem& it, const NsScalars& q, char* Xh, char* Xl, uint32_t blk,
+                                          bool turn) {
+  const int rows = it.rows, cols = it.cols;
+  const T* const in = static_cast<const T*>(it.in);
+  float* const mom = it.mom;
+  const int64_t ld_in = it.ld_in, ld_mom = it.ld_mom;
+  const float mu = q.mu, nu = q.nu;
+  const bool nesterov = q.nesterov;
+  double ss = 0.0;
+  float g[8], m[8];
+  Unit u(cols);
+  if (u.r0 < rows) {
+    unit_load(in, ld_in, u, rows, cols, g);
+    if (MOM) unit_load(mom, ld_mom, u, rows, cols, m);
+  }
+#pragma unroll 1
+  while (u.r0 < rows) {
+    float g2[8], m2[8];
+    Unit t = u;
+    t.next();
+    if (t.r0 < rows) {
+      unit_load(in, ld_in, t, rows, cols, g2);
+      if (MOM) unit_load(mom, ld_mom, t, rows, cols, m2);
+    }
+    if (MOM) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        m[k] = fmaf(mu, m[k], nu * g[k]);
+        g[k] = nesterov ? fmaf(mu, m[k], nu * g[k]) : m[k];
+      }
+      unit_store(mom, ld_mom, u, rows, cols, m);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss = fma((double)g[k], (double)g[k], ss);
+    if (u.c < cols) {   // rows past the matrix get the zeros that are there already
+      if (turn) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t x = __float_as_uint(g[2 * k]), y = __float_as_uint(g[2 * k + 1]);
+          h[k] = __byte_perm(x, y, 0x7632);
+          l[k] = __byte_perm(x, y, 0x5410);
+        }
+        const uint32_t o = unit_chunk(u, blk);
+        *reinterpret_cast<uint4*>(Xh + o) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(Xl + o) = make_uint4(l[0], l[1], l[2], l[3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t o = unit_row(u, blk, k), x = __float_as_uint(g[k]);
+          *reinterpret_cast<uint16_t*>(Xh + o) = (uint16_t)(x >> 16);
+          *reinterpret_cast<uint16_t*>(Xl + o) = (uint16_t)x;
+        }
+      }
+    }
+    u = t;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      g[k] = g2[k];
+      if (MOM) m[k] = m2[k];
+    }
+  }
+  return ss;
+}
+
+// The tiles (raw) to the result, or the weight moved by them.
+template <typename T, bool MOM>
+__device__ __forceinline__ void give_out(const NsItem& it, const NsScalars& q, const char* Xh, const char* Xl,
+                                         uint32_t blk, bool turn) {
+  const int rows = it.rows, cols = it.cols;
+  T* const out = static_cast<T*>(it.out);
+  const int64_t ld = it.ld_out;
+  float keep = 0.f, move = 0.f;
+  if (MOM) ns_rates(it, q, keep, move);
+  float w[8];
+  Unit u(cols);
+  if (MOM && u.r0 < rows) unit_load(out, ld, u, rows, cols, w);
+#pragma unroll 1
+  while (u.r0 < rows) {
+    float w2[8], v[8];
+    Unit t = u;
+    t.next();
+    if (MOM && t.r0 < rows) unit_load(out, ld, t, rows, cols, w2);
+    if (u.c < cols) {
+      if (turn) {
+        const uint32_t o = unit_chunk(u, blk);
+        const uint4 h = *reinterpret_cast<const uint4*>(Xh + o), l = *reinterpret_cast<const uint4*>(Xl + o);
+        const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[2 * k] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x5410));
+          v[2 * k + 1] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x7632));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t o = unit_row(u, blk, k);
+          v[k] = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(Xh + o) << 16 |
+                                 *reinterpret_cast<const uint16_t*>(Xl + o));
+        }
+      }
+      if (MOM)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = fmaf(move, v[k], keep * w[k]);
+      unit_store(out, ld, u, rows, cols, v);
+    }
+    u = t;
+    if (MOM)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = w2[k];
+  }
+}
 
 // Thread-uniform wait for the commit on `bar`; false when it ran out.
 __device__ __forceinline__ bool wait_commit(uint64_t* bar, uint32_t parity) {
@@ -161,29 +341,11 @@ __global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_cons
   }
   pdl_enter();
 
-  // ---- U, its norm (squares added in float64: no overflow or underflow at any
-  // scale of the gradient), X0.  Element i is thread i % kThreads's in both
-  // passes; kBatch elements are loaded before any of them is used.
-  Walk walk(it, tid);
-  double ss = 0.0;
-  for (; walk.any(); walk.next()) {
-    float g[kBatch], mo[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      g[k] = walk.has(k) ? ns_load(it.in, it.dtype, walk.r[k] * it.ld_in + walk.c[k]) : 0.f;
-      mo[k] = it.mom && walk.has(k) ? it.mom[walk.r[k] * it.ld_mom + walk.c[k]] : 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      float u = g[k];
-      if (it.mom && walk.has(k)) {
-        const float mv = ns_momentum(q, g[k], mo[k]);
-        it.mom[walk.r[k] * it.ld_mom + walk.c[k]] = mv;
-        u = ns_update(q, g[k], mv);
-      }
-      ss += (double)u * u;
-    }
-  }
+  __syncthreads();
+  double ss = it.mom                            ? take_in<float, true>(it, q, Xh, Xl, R * 128, turn)
+              : it.dtype == EGNN_DTYPE_F32  ? take_in<float, false>(it, q, Xh, Xl, R * 128, turn)
+              : it.dtype == EGNN_DTYPE_BF16 ? take_in<__nv_bfloat16, false>(it, q, Xh, Xl, R * 128, turn)
+                                            : take_in<__half, false>(it, q, Xh, Xl, R * 128, turn);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
   if (lane == 0) red[warp] = ss;
@@ -195,53 +357,47 @@ __global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_cons
 #pragma unroll
   for (int k = 0; k < kWarps; ++k) ss += red[k];
   const double inv = 1.0 / (sqrt(ss) + q.eps);
-  for (walk = Walk(it, tid); walk.any(); walk.next()) {
-    float u[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      u[k] = walk.has(k) ? ns_load(it.in, it.dtype, walk.r[k] * it.ld_in + walk.c[k]) : 0.f;
-      if (it.mom && walk.has(k)) u[k] = ns_update(q, u[k], it.mom[walk.r[k] * it.ld_mom + walk.c[k]]);
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (!walk.has(k)) continue;
-      const float v = (float)(u[k] * inv) * q.sx;
-      const uint32_t o = turn ? sw128_offset(walk.c[k], walk.r[k], R) : sw128_offset(walk.r[k], walk.c[k], R);
-      const __half h = __float2half_rn(v);
-      *reinterpret_cast<__half*>(Xh + o) = h;
-      *reinterpret_cast<__half*>(Xl + o) = __float2half_rn(v - __half2float(h));
-    }
-  }
-  hand_over();
-
-  // warp w reads accumulator lanes 32 (w % 4) .. + 31 = tile rows, and of each
-  // group of four 32-column pieces the (w / 4)-th
+  // a power of two first, so that the rest of the scale is a float32 at any norm
+  const float pre = inv > 1.0 ? 0x1p64f : inv < 0x1p-64 ? 0x1p-64f : 1.f, f = (float)(inv / (double)pre);
+  // warp w owns tile rows 32 (w % 4) .. + 31, which are its accumulator lanes,
+  // and of each group of four 32-column pieces the (w / 4)-th
   const int row = (warp & 3) * 32 + lane, piece = warp >> 2;
   const bool rows_here = (warp & 3) * 32 < R;
   const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  if (rows_here)
+    for (int c0 = piece * 32; c0 < n16; c0 += 128) {
+      float v[32];
+      load_raw32(Xh, Xl, R, row, c0, v);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] = v[k] * pre * f;
+      if (q.steps == 0) {
+        store_raw32(Xh, Xl, R, row, c0, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= q.sx;
+        store_pairs32(Xh, Xl, R, row, c0, v);
+      }
+    }
+  hand_over();
+
   const uint32_t tA = 0, tAA = 128;
   const uint32_t idesc_m = make_idesc_f16(128, m16, 0, 0);
   const float fA = q.sa / (q.sx * q.sx);                    // accumulator -> A scaled
   const float fbA = q.b * q.sb / (q.sx * q.sx), fcAA = q.c * q.sb / (q.sa * q.sa);
-  const float fX = 1.f / q.sb;
+  const float fX = 1.f / q.sb, back = 1.f / q.sx;
   const int n_slots = (n16 + kSlotCols - 1) / kSlotCols;
+  const int uwarp = __shfl_sync(0xffffffffu, warp, 0);   // the same, known to be uniform
   uint32_t phase = 0, pending = 0;   // bit k: parity of bar[k]; a commit on it not yet waited for
   bool ok = true;
 
   // X' columns [128 k, 128 k + 128) into slot k % kSlots
   auto issue_update = [&](int k) {
     pending |= 1u << (k % kSlots);
-    if (tid != 0) return;
+    if (uwarp != 0) return;
     const int c0 = k * kSlotCols, N = min(kSlotCols, n16 - c0);
-    const uint32_t d = tmem + (k % kSlots) * kSlotCols;
-    const uint32_t idesc = make_idesc_f16(128, N, 0, 1);
-    for (int p = 0; p < 3; ++p) {
-      const char* L = p == 0 ? Al : Ah;
-      const char* X = p == 1 ? Xl : Xh;
-      for (int kk = 0; kk < m16 / 16; ++kk)
-        mma_f16(d, desc_k(L, R, kk), desc_mn(X, R, c0, kk), idesc, (p | kk) ? 1u : 0u);
-    }
-    mma_commit(&bar[k % kSlots]);
+    const uint32_t one = elect_one();
+    issue3<true>(one, tmem + (k % kSlots) * kSlotCols, Ah, Al, Xh, Xl, R, c0, m16 / 16, make_idesc_f16(128, N, 0, 1));
+    if (one) mma_commit(&bar[k % kSlots]);
   };
   auto wait_slot = [&](int k) {
     const bool good = wait_commit(&bar[k], (phase >> k) & 1u);
@@ -254,14 +410,10 @@ __global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_cons
 
 #pragma unroll 1
   for (int step = 0; step < q.steps && ok; ++step) {
-    if (tid == 0) {
-      for (int p = 0; p < 3; ++p) {
-        const char* L = p == 0 ? Xl : Xh;
-        const char* Rr = p == 1 ? Xl : Xh;
-        for (int kk = 0; kk < n16 / 16; ++kk)
-          mma_f16(tmem + tA, desc_k(L, R, kk), desc_k(Rr, R, kk), idesc_m, (p | kk) ? 1u : 0u);
-      }
-      mma_commit(&bar[0]);
+    if (uwarp == 0) {
+      const uint32_t one = elect_one();
+      issue3<false>(one, tmem + tA, Xh, Xl, Xh, Xl, R, 0, n16 / 16, idesc_m);
+      if (one) mma_commit(&bar[0]);
     }
     pending |= 1u;
     if (!(ok = wait_slot(0))) break;
@@ -273,14 +425,10 @@ __global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_cons
       store_pairs32(Ah, Al, R, row, piece * 32, v);
     }
     hand_over();
-    if (tid == 0) {
-      for (int p = 0; p < 3; ++p) {
-        const char* L = p == 0 ? Al : Ah;
-        const char* Rr = p == 1 ? Al : Ah;
-        for (int kk = 0; kk < m16 / 16; ++kk)
-          mma_f16(tmem + tAA, desc_k(L, R, kk), desc_k(Rr, R, kk), idesc_m, (p | kk) ? 1u : 0u);
-      }
-      mma_commit(&bar[0]);
+    if (uwarp == 0) {
+      const uint32_t one = elect_one();
+      issue3<false>(one, tmem + tAA, Ah, Al, Ah, Al, R, 0, m16 / 16, idesc_m);
+      if (one) mma_commit(&bar[0]);
     }
     pending |= 1u;
     if (!(ok = wait_slot(0))) break;
@@ -303,7 +451,13 @@ __global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_cons
         load_pairs32(Xh, Xl, R, row, c0, x);
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = fmaf(q.a, x[j], fX * v[j]);
-        store_pairs32(Xh, Xl, R, row, c0, v);
+        if (step + 1 < q.steps) {
+          store_pairs32(Xh, Xl, R, row, c0, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= back;
+          store_raw32(Xh, Xl, R, row, c0, v);
+        }
       }
       if (k + kSlots < n_slots) {   // the slot is free once every thread has read it
         fence_before_sync();
@@ -322,25 +476,10 @@ __global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_cons
         if (pending >> k & 1u) mbar_wait(&bar[k], (phase >> k) & 1u);
     }
   } else {
-    const float back = 1.f / q.sx;
-    float keep = 0.f, move = 0.f;
-    if (it.mom) ns_rates(it, q, keep, move);
-    for (walk = Walk(it, tid); walk.any(); walk.next()) {
-      float w[kBatch];
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k)
-        w[k] = it.mom && walk.has(k) ? static_cast<const float*>(it.out)[walk.r[k] * it.ld_out + walk.c[k]] : 0.f;
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (!walk.has(k)) continue;
-        const uint32_t o = turn ? sw128_offset(walk.c[k], walk.r[k], R) : sw128_offset(walk.r[k], walk.c[k], R);
-        const float v = (__half2float(*reinterpret_cast<const __half*>(Xh + o)) +
-                         __half2float(*reinterpret_cast<const __half*>(Xl + o))) * back;
-        const int64_t io = walk.r[k] * it.ld_out + walk.c[k];
-        if (it.mom) static_cast<float*>(it.out)[io] = fmaf(move, v, keep * w[k]);
-        else ns_store(it.out, it.dtype, io, v);
-      }
-    }
+    if (it.mom) give_out<float, true>(it, q, Xh, Xl, R * 128, turn);
+    else if (it.dtype == EGNN_DTYPE_F32) give_out<float, false>(it, q, Xh, Xl, R * 128, turn);
+    else if (it.dtype == EGNN_DTYPE_BF16) give_out<__nv_bfloat16, false>(it, q, Xh, Xl, R * 128, turn);
+    else give_out<__half, false>(it, q, Xh, Xl, R * 128, turn);
   }
   fence_before_sync();
   __syncthreads();
