@@ -31,6 +31,7 @@ using namespace tc;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSlots = 4, kSlotCols = 128;   // X' accumulators in tensor memory
+constexpr int kMaxChunks = 16;               // of 128 columns of X: at most 27 column blocks fit
 constexpr int kSmemMax = 232448 - 1024;      // a block's shared memory less the static part
 
 // Rows of a tile: all column blocks are `rows` x 128 bytes.
@@ -43,10 +44,10 @@ __host__ __device__ inline size_t smem_bytes(int m, int n) {
   return (size_t)((n + 63) / 64 + (m + 63) / 64) * R * 256 + (128 - R) * 128 + 1024;
 }
 
-// hi and lo tiles at (row, c0 .. c0 + 31) <- v.
-__device__ __forceinline__ void store_pairs32(char* hi, char* lo, int R, int row, int c0, const float (&v)[32]) {
+// hi and lo tiles at (row, c0 .. c0 + 15) <- v[at .. at + 15].
+__device__ __forceinline__ void store_pairs16(char* hi, char* lo, int R, int row, int c0, const float* v) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
     uint32_t h[4], l[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -81,9 +82,9 @@ __device__ __forceinline__ void load_pairs32(const char* hi, const char* lo, int
 
 // The same places hold a float32's upper and lower 16 bits before the first
 // product and after the last.
-__device__ __forceinline__ void store_raw32(char* hi, char* lo, int R, int row, int c0, const float (&v)[32]) {
+__device__ __forceinline__ void store_raw16(char* hi, char* lo, int R, int row, int c0, const float* v) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 2; ++j) {
     uint32_t h[4], l[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -110,35 +111,27 @@ __device__ __forceinline__ void load_raw32(const char* hi, const char* lo, int R
   }
 }
 
-// Issues D (+)= L R over nk K-steps of 16.  L is K-major; R is K-major, or
-// MN-major from column c0 on.  Tiles of `rows` rows; only the address field of
-// the descriptors moves.
+// Issues D (+)= L R over the K-steps h, h + 2, h + 4, h + 6 (those below nk) of
+// 128 columns of L.  L is K-major from descriptor l, R K-major too or MN-major
+// from r; blk16 is a column block in descriptor units.
 template <bool MN>
-__device__ __forceinline__ void issue(uint32_t one, uint32_t d, const char* L, const char* Rt, int rows, int c0, int nk, uint32_t idesc,
-                                      bool accumulate) {
-  const uint32_t blk = rows * 128;
-  uint64_t l = make_desc(smem_u32(L), 16, 1024);
-  uint64_t r = MN ? make_desc(smem_u32(Rt) + (c0 >> 6) * blk, blk, 1024) : make_desc(smem_u32(Rt), 16, 1024);
-  uint32_t acc = accumulate;
-#pragma unroll 1
-  for (int k0 = 0; k0 < nk; k0 += 4) {
+__device__ __forceinline__ void issue(uint32_t one, uint32_t d, uint64_t l, uint64_t r, uint32_t blk16, int h, int nk,
+                                      uint32_t idesc, uint32_t accumulate) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (k0 + j < nk) {
-        mma_f16_elected(one, d, l + 2 * j, r + (MN ? 128 : 2) * j, idesc, acc);
-        acc = 1;
-      }
-    l += blk >> 4;
-    r += MN ? 512 : blk >> 4;
-  }
+  for (int p = 0; p < 4; ++p)
+    if (2 * p + h < nk) {
+      const uint32_t k_major = (p >> 1) * blk16 + (p & 1) * 4 + h * 2;
+      mma_f16_elected(one, d, l + k_major, r + (MN ? (2 * p + h) * 128 : k_major), idesc, accumulate);
+      accumulate = 1;
+    }
 }
 // lo hi + hi lo + hi hi, in this order.
 template <bool MN>
-__device__ __forceinline__ void issue3(uint32_t one, uint32_t d, const char* Lh, const char* Ll, const char* Rh, const char* Rl, int rows,
-                                       int c0, int nk, uint32_t idesc) {
-  issue<MN>(one, d, Ll, Rh, rows, c0, nk, idesc, false);
-  issue<MN>(one, d, Lh, Rl, rows, c0, nk, idesc, true);
-  issue<MN>(one, d, Lh, Rh, rows, c0, nk, idesc, true);
+__device__ __forceinline__ void issue3(uint32_t one, uint32_t d, uint64_t lh, uint64_t ll, uint64_t rh, uint64_t rl,
+                                       uint32_t blk16, int h, int nk, uint32_t idesc, uint32_t accumulate) {
+  issue<MN>(one, d, ll, rh, blk16, h, nk, idesc, accumulate);
+  issue<MN>(one, d, lh, rl, blk16, h, nk, idesc, 1);
+  issue<MN>(one, d, lh, rh, blk16, h, nk, idesc, 1);
 }
 
 // A warp's share of a matrix in global memory: units of 8 rows x 32 columns,
@@ -299,29 +292,51 @@ __device__ __forceinline__ void give_out(const NsItem& it, const NsScalars& q, c
   }
 }
 
-// Thread-uniform wait for the commit on `bar`; false when it ran out.
-__device__ __forceinline__ bool wait_commit(uint64_t* bar, uint32_t parity) {
-  const bool ok = mbar_wait(bar, parity);
-  const bool bad = __syncthreads_or(!ok);
+struct Barriers {
+  uint64_t a_done, aa_done;              // commits of X X^T and A A
+  uint64_t slot_done[kSlots];            // commits of X' columns
+  uint64_t a_ready[2], b_ready[2];       // halves of the A and B tiles are written
+  uint64_t x_ready[kMaxChunks][2];       // halves of each 128 columns of X
+  uint64_t drained;
+};
+
+// Bounded wait, the same answer in the whole warp; false when it or another
+// warp's wait ran out.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+  bool ok = false;
+  for (uint32_t i = 0; i < (1u << 22) && !ok; ++i) {
+    ok = mbar_try_wait(bar, parity & 1u);
+    if (!ok && (i & 255u) == 255u && *gave_up) break;
+  }
+  ok = __all_sync(0xffffffffu, ok);
+  if (!ok) *gave_up = 1;
   fence_after_sync();
-  return !bad;
+  return ok;
 }
-// Tile writes and accumulator reads done by every thread -> the next products may go.
-__device__ __forceinline__ void hand_over() {
+// This warp's tile writes and accumulator reads are done.
+__device__ __forceinline__ void arrive(uint64_t* bar) {
   fence_proxy_async();
   fence_before_sync();
-  __syncthreads();
-  fence_after_sync();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0)
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-__global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_constant__ NsBatch batch,
-                                                               const __grid_constant__ NsScalars q) {
+// Warps 0 .. 15 take the matrix in, turn accumulators into operand tiles and
+// give the result out; warp 16 issues the products.  Operands are handed over
+// in halves (even and odd K-steps), so that products run while the second
+// half is still being written, and X X^T of the next step runs while the last
+// columns of X' are.
+__global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid_constant__ NsBatch batch,
+                                                                    const __grid_constant__ NsScalars q) {
   extern __shared__ char raw[];
-  __shared__ uint64_t bar[kSlots];
+  __shared__ Barriers bar;
   __shared__ uint32_t tmem_s;
+  __shared__ int gave_up_s;
   __shared__ double red[kWarps];
   const NsItem& it = batch.it[blockIdx.x];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // known to be uniform
   const bool turn = it.rows > it.cols;
   const int m = turn ? it.cols : it.rows, n = turn ? it.rows : it.cols;
   const int R = tile_rows(m);
@@ -331,164 +346,215 @@ __global__ void __launch_bounds__(kThreads, 1) ns_fused_kernel(const __grid_cons
   char* const Xl = Xh + xt;
   char* const Ah = Xl + xt;
   char* const Al = Ah + at;
+  volatile int* const gave_up = &gave_up_s;
+  const int chunks = (n16 + kSlotCols - 1) / kSlotCols;
 
   // padding rows and columns of X are zeros, and every product keeps them so
-  for (int i = tid; i < 2 * xt / 16; i += kThreads) reinterpret_cast<uint4*>(Xh)[i] = make_uint4(0, 0, 0, 0);
-  if (warp == 0) tmem_alloc(&tmem_s, 512);
-  if (tid == 0) {
-    for (int k = 0; k < kSlots; ++k) mbar_init(&bar[k], 1);
-    fence_mbar_init();
+  for (int i = tid; i < 2 * xt / 16; i += kThreads + 32) reinterpret_cast<uint4*>(Xh)[i] = make_uint4(0, 0, 0, 0);
+  if (warp == kWarps) {
+    tmem_alloc(&tmem_s, 512);
+    if (lane == 0) {
+      gave_up_s = 0;
+      mbar_init(&bar.a_done, 1);
+      mbar_init(&bar.aa_done, 1);
+      mbar_init(&bar.drained, 1);
+      for (int k = 0; k < kSlots; ++k) mbar_init(&bar.slot_done[k], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bar.a_ready[h], kWarps);
+        mbar_init(&bar.b_ready[h], kWarps);
+        for (int k = 0; k < chunks; ++k) mbar_init(&bar.x_ready[k][h], kWarps);
+      }
+      fence_mbar_init();
+    }
   }
   pdl_enter();
-
   __syncthreads();
-  double ss = it.mom                            ? take_in<float, true>(it, q, Xh, Xl, R * 128, turn)
-              : it.dtype == EGNN_DTYPE_F32  ? take_in<float, false>(it, q, Xh, Xl, R * 128, turn)
-              : it.dtype == EGNN_DTYPE_BF16 ? take_in<__nv_bfloat16, false>(it, q, Xh, Xl, R * 128, turn)
-                                            : take_in<__half, false>(it, q, Xh, Xl, R * 128, turn);
+  if (warp < kWarps) {
+    double ss = it.mom                            ? take_in<float, true>(it, q, Xh, Xl, R * 128, turn)
+                : it.dtype == EGNN_DTYPE_F32  ? take_in<float, false>(it, q, Xh, Xl, R * 128, turn)
+                : it.dtype == EGNN_DTYPE_BF16 ? take_in<__nv_bfloat16, false>(it, q, Xh, Xl, R * 128, turn)
+                                              : take_in<__half, false>(it, q, Xh, Xl, R * 128, turn);
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-  if (lane == 0) red[warp] = ss;
+    for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    if (lane == 0) red[warp] = ss;
+  }
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = tmem_s;
-  ss = 0.0;
-#pragma unroll
-  for (int k = 0; k < kWarps; ++k) ss += red[k];
-  const double inv = 1.0 / (sqrt(ss) + q.eps);
-  // a power of two first, so that the rest of the scale is a float32 at any norm
-  const float pre = inv > 1.0 ? 0x1p64f : inv < 0x1p-64 ? 0x1p-64f : 1.f, f = (float)(inv / (double)pre);
-  // warp w owns tile rows 32 (w % 4) .. + 31, which are its accumulator lanes,
-  // and of each group of four 32-column pieces the (w / 4)-th
-  const int row = (warp & 3) * 32 + lane, piece = warp >> 2;
-  const bool rows_here = (warp & 3) * 32 < R;
-  const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  if (rows_here)
-    for (int c0 = piece * 32; c0 < n16; c0 += 128) {
-      float v[32];
-      load_raw32(Xh, Xl, R, row, c0, v);
-#pragma unroll
-      for (int k = 0; k < 32; ++k) v[k] = v[k] * pre * f;
-      if (q.steps == 0) {
-        store_raw32(Xh, Xl, R, row, c0, v);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] *= q.sx;
-        store_pairs32(Xh, Xl, R, row, c0, v);
-      }
-    }
-  hand_over();
+  const uint32_t tA = tmem, tAA = tmem + kSlotCols;   // the slots 0 and 1, which hold X' only after B is made
 
-  const uint32_t tA = 0, tAA = 128;
-  const uint32_t idesc_m = make_idesc_f16(128, m16, 0, 0);
-  const float fA = q.sa / (q.sx * q.sx);                    // accumulator -> A scaled
-  const float fbA = q.b * q.sb / (q.sx * q.sx), fcAA = q.c * q.sb / (q.sa * q.sa);
-  const float fX = 1.f / q.sb, back = 1.f / q.sx;
-  const int n_slots = (n16 + kSlotCols - 1) / kSlotCols;
-  const int uwarp = __shfl_sync(0xffffffffu, warp, 0);   // the same, known to be uniform
-  uint32_t phase = 0, pending = 0;   // bit k: parity of bar[k]; a commit on it not yet waited for
-  bool ok = true;
-
-  // X' columns [128 k, 128 k + 128) into slot k % kSlots
-  auto issue_update = [&](int k) {
-    pending |= 1u << (k % kSlots);
-    if (uwarp != 0) return;
-    const int c0 = k * kSlotCols, N = min(kSlotCols, n16 - c0);
+  if (warp == kWarps) {
     const uint32_t one = elect_one();
-    issue3<true>(one, tmem + (k % kSlots) * kSlotCols, Ah, Al, Xh, Xl, R, c0, m16 / 16, make_idesc_f16(128, N, 0, 1));
-    if (one) mma_commit(&bar[k % kSlots]);
-  };
-  auto wait_slot = [&](int k) {
-    const bool good = wait_commit(&bar[k], (phase >> k) & 1u);
-    if (good) {
-      phase ^= 1u << k;
-      pending &= ~(1u << k);
-    }
-    return good;
-  };
-
+    const uint32_t blk16 = R * 8;
+    const uint32_t idesc_m = make_idesc_f16(128, m16, 0, 0);
+    const int nk = n16 >> 4, mk = m16 >> 4;
+    const uint64_t xh = make_desc(smem_u32(Xh), 16, 1024), xl = make_desc(smem_u32(Xl), 16, 1024);
+    const uint64_t ah = make_desc(smem_u32(Ah), 16, 1024), al = make_desc(smem_u32(Al), 16, 1024);
+    const uint64_t xh_mn = make_desc(smem_u32(Xh), R * 128, 1024), xl_mn = make_desc(smem_u32(Xl), R * 128, 1024);
+    bool ok = true;
 #pragma unroll 1
-  for (int step = 0; step < q.steps && ok; ++step) {
-    if (uwarp == 0) {
-      const uint32_t one = elect_one();
-      issue3<false>(one, tmem + tA, Xh, Xl, Xh, Xl, R, 0, n16 / 16, idesc_m);
-      if (one) mma_commit(&bar[0]);
-    }
-    pending |= 1u;
-    if (!(ok = wait_slot(0))) break;
-    if (rows_here && piece * 32 < m16) {
-      float v[32];
-      tmem_ld32(tl + tA + piece * 32, v);
-#pragma unroll
-      for (int k = 0; k < 32; ++k) v[k] *= fA;
-      store_pairs32(Ah, Al, R, row, piece * 32, v);
-    }
-    hand_over();
-    if (uwarp == 0) {
-      const uint32_t one = elect_one();
-      issue3<false>(one, tmem + tAA, Ah, Al, Ah, Al, R, 0, m16 / 16, idesc_m);
-      if (one) mma_commit(&bar[0]);
-    }
-    pending |= 1u;
-    if (!(ok = wait_slot(0))) break;
-    if (rows_here && piece * 32 < m16) {
-      float v[32], w[32];
-      tmem_ld32(tl + tA + piece * 32, v);
-      tmem_ld32(tl + tAA + piece * 32, w);
-#pragma unroll
-      for (int k = 0; k < 32; ++k) v[k] = fmaf(fbA, v[k], fcAA * w[k]);
-      store_pairs32(Ah, Al, R, row, piece * 32, v);
-    }
-    hand_over();
-    for (int k = 0; k < min(n_slots, kSlots); ++k) issue_update(k);
-    for (int k = 0; k < n_slots; ++k) {
-      if (!(ok = wait_slot(k % kSlots))) break;
-      const int c0 = k * kSlotCols + piece * 32;
-      if (rows_here && c0 < n16) {
-        float v[32], x[32];
-        tmem_ld32(tl + (k % kSlots) * kSlotCols + piece * 32, v);
-        load_pairs32(Xh, Xl, R, row, c0, x);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = fmaf(q.a, x[j], fX * v[j]);
-        if (step + 1 < q.steps) {
-          store_pairs32(Xh, Xl, R, row, c0, v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= back;
-          store_raw32(Xh, Xl, R, row, c0, v);
+    for (int step = 0; step < q.steps && ok; ++step) {
+      // a slot used more than once: its last X' columns have to be read before A goes there
+      for (int k = kSlots; k < chunks && ok; ++k)
+        ok = wait_bar(&bar.x_ready[k][0], step, gave_up) && wait_bar(&bar.x_ready[k][1], step, gave_up);
+#pragma unroll 1
+      for (int k = 0; k < chunks && ok; ++k)
+#pragma unroll 1
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (!(ok = wait_bar(&bar.x_ready[k][h], step, gave_up))) break;
+          const uint32_t o = 2 * k * blk16;
+          issue3<false>(one, tA, xh + o, xl + o, xh + o, xl + o, blk16, h, nk - 8 * k, idesc_m, k | h);
+        }
+      if (!ok) break;
+      if (one) mma_commit(&bar.a_done);
+#pragma unroll 1
+      for (int h = 0; h < 2 && ok; ++h) {
+        if (!(ok = wait_bar(&bar.a_ready[h], step, gave_up))) break;
+        issue3<false>(one, tAA, ah, al, ah, al, blk16, h, mk, idesc_m, h);
+      }
+      if (!ok) break;
+      if (one) mma_commit(&bar.aa_done);
+      // X' columns [128 k, 128 k + 128) into slot k % kSlots
+      if (!(ok = wait_bar(&bar.b_ready[0], step, gave_up))) break;
+#pragma unroll 1
+      for (int k0 = 0; k0 < chunks && ok; k0 += kSlots) {
+        const int k1 = min(chunks, k0 + kSlots);
+#pragma unroll 1
+        for (int h = 0; h < 2 && ok; ++h) {
+          if (h == 1 && k0 == 0 && !(ok = wait_bar(&bar.b_ready[1], step, gave_up))) break;
+#pragma unroll 1
+          for (int k = k0; k < k1 && ok; ++k) {
+            // a slot that was used in this step is free once X' has been read out of it
+            if (h == 0 && k >= kSlots &&
+                !(ok = wait_bar(&bar.x_ready[k - kSlots][0], step + 1, gave_up) &&
+                       wait_bar(&bar.x_ready[k - kSlots][1], step + 1, gave_up)))
+              break;
+            const uint32_t o = 2 * k * blk16;
+            issue3<true>(one, tmem + (k - k0) * kSlotCols, ah, al, xh_mn + o, xl_mn + o, blk16, h, mk,
+                         make_idesc_f16(128, min(kSlotCols, n16 - k * kSlotCols), 0, 1), h);
+            if (h == 1 || mk == 1) {
+              if (one) mma_commit(&bar.slot_done[k - k0]);
+            }
+          }
+          if (mk == 1) break;
         }
       }
-      if (k + kSlots < n_slots) {   // the slot is free once every thread has read it
-        fence_before_sync();
-        __syncthreads();
-        fence_after_sync();
-        issue_update(k + kSlots);
+    }
+    // nothing may be in flight when the tensor memory goes
+    if (one) mma_commit(&bar.drained);
+    wait_bar(&bar.drained, 0, gave_up);
+  } else {
+    double ss = 0.0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) ss += red[k];
+    const double inv = 1.0 / (sqrt(ss) + q.eps);
+    // a power of two first, so that the rest of the scale is a float32 at any norm
+    const float pre = inv > 1.0 ? 0x1p64f : inv < 0x1p-64 ? 0x1p-64f : 1.f, f = (float)(inv / (double)pre);
+    // warp w owns tile rows 32 (w % 4) .. + 31, which are its accumulator lanes,
+    // and of each group of four 32-column pieces the (w / 4)-th
+    const int row = (warp & 3) * 32 + lane, piece = warp >> 2;
+    const bool rows_here = (warp & 3) * 32 < R;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    for (int k = 0; k < chunks; ++k) {
+      const int c0 = k * kSlotCols + piece * 32;
+      float v[32];
+      if (rows_here && c0 < n16) {
+        load_raw32(Xh, Xl, R, row, c0, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = v[j] * pre * f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (rows_here && c0 < n16) {
+          if (q.steps == 0) {
+            store_raw16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+          } else {
+#pragma unroll
+            for (int j = 16 * h; j < 16 * h + 16; ++j) v[j] *= q.sx;
+            store_pairs16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+          }
+        }
+        arrive(&bar.x_ready[k][h]);
       }
     }
-    hand_over();
+
+    const float fA = q.sa / (q.sx * q.sx);                    // accumulator -> A scaled
+    const float fbA = q.b * q.sb / (q.sx * q.sx), fcAA = q.c * q.sb / (q.sa * q.sa);
+    const float fX = 1.f / q.sb, back = 1.f / q.sx;
+    const bool a_here = rows_here && piece * 32 < m16;
+    bool ok = true;
+#pragma unroll 1
+    for (int step = 0; step < q.steps && ok; ++step) {
+      float v[32], w[32];
+      if (!(ok = wait_bar(&bar.a_done, step, gave_up))) break;
+      if (a_here) {
+        tmem_ld32(tA + lanes + piece * 32, v);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= fA;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (a_here) store_pairs16(Ah, Al, R, row, piece * 32 + 16 * h, v + 16 * h);
+        arrive(&bar.a_ready[h]);
+      }
+      if (!(ok = wait_bar(&bar.aa_done, step, gave_up))) break;
+      if (a_here) {
+        tmem_ld32(tA + lanes + piece * 32, v);
+        tmem_ld32(tAA + lanes + piece * 32, w);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = fmaf(fbA, v[k], fcAA * w[k]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (a_here) store_pairs16(Ah, Al, R, row, piece * 32 + 16 * h, v + 16 * h);
+        arrive(&bar.b_ready[h]);
+      }
+#pragma unroll 1
+      for (int k = 0; k < chunks; ++k) {
+        const int slot = k % kSlots, uses = (chunks - slot + kSlots - 1) / kSlots;   // of this slot in a step
+        if (!(ok = wait_bar(&bar.slot_done[slot], step * uses + k / kSlots, gave_up))) break;
+        const int c0 = k * kSlotCols + piece * 32;
+        const bool here = rows_here && c0 < n16;
+        if (here) {
+          tmem_ld32(tmem + lanes + slot * kSlotCols + piece * 32, v);
+          load_pairs32(Xh, Xl, R, row, c0, w);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(q.a, w[j], fX * v[j]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (here) {
+            if (step + 1 < q.steps) {
+              store_pairs16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+            } else {
+#pragma unroll
+              for (int j = 16 * h; j < 16 * h + 16; ++j) v[j] *= back;
+              store_raw16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+            }
+          }
+          arrive(&bar.x_ready[k][h]);
+        }
+      }
+    }
   }
 
-  if (!ok) {
-    if (tid == 0) {   // what is still in flight ends before the tensor memory goes
-      atomicAdd(&g_ns_fused_timeouts, 1);
-      for (int k = 0; k < kSlots; ++k)
-        if (pending >> k & 1u) mbar_wait(&bar[k], (phase >> k) & 1u);
-    }
-  } else {
+  fence_before_sync();
+  __syncthreads();
+  if (warp == kWarps) {
+    if (lane == 0 && *gave_up) atomicAdd(&g_ns_fused_timeouts, 1);
+    tmem_dealloc(tmem, 512);
+  } else if (!*gave_up) {
     if (it.mom) give_out<float, true>(it, q, Xh, Xl, R * 128, turn);
     else if (it.dtype == EGNN_DTYPE_F32) give_out<float, false>(it, q, Xh, Xl, R * 128, turn);
     else if (it.dtype == EGNN_DTYPE_BF16) give_out<__nv_bfloat16, false>(it, q, Xh, Xl, R * 128, turn);
     else give_out<__half, false>(it, q, Xh, Xl, R * 128, turn);
   }
-  fence_before_sync();
-  __syncthreads();
-  if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace
 
-bool ns_fused_fits(int m, int n) { return m <= 128 && smem_bytes(m, n) <= (size_t)kSmemMax; }
+bool ns_fused_fits(int m, int n) { return m <= 128 && n <= kMaxChunks * kSlotCols && smem_bytes(m, n) <= (size_t)kSmemMax; }
 
 int ns_fused(const NsBatch& b, const NsScalars& q, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
@@ -501,7 +567,7 @@ int ns_fused(const NsBatch& b, const NsScalars& q, cudaStream_t s) {
   for (int i = 0; i < b.count; ++i)
     smem = std::max(smem, smem_bytes(std::min(b.it[i].rows, b.it[i].cols), std::max(b.it[i].rows, b.it[i].cols)));
   TimerScope ts("newton_schulz", s);
-  EGNN_CHECK_CUDA(launch_pdl(ns_fused_kernel, dim3(b.count), dim3(kThreads), smem, s, b, q));
+  EGNN_CHECK_CUDA(launch_pdl(ns_fused_kernel, dim3(b.count), dim3(kThreads + 32), smem, s, b, q));
   EGNN_CHECK_LAUNCH();
   return EGNN_OK;
 }
