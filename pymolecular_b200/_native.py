@@ -209,9 +209,12 @@ def ptr(t) -> int | None:
 
 
 def stream_ptr(stream=None) -> int:
+    """Handle of `stream`, or of the current stream of the current device."""
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # a tenth of the cost of making a Stream object
+    return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
 
 
 def device_of(t):

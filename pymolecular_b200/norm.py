@@ -20,14 +20,42 @@ DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.fl
 def _forward(x, weight, bias, eps, stats):
     """y and, where asked for, the (rows, 2) mean and 1 / sqrt(var + eps)."""
     rows, cols = x.shape
-    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     kept = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if stats else None
     p = weight if weight is not None else bias
     with nat.device_of(x):
-        nat.check(nat.lib().egnn_layer_norm_fwd(rows, cols, nat.ptr(x), x.stride(0), DTYPES[x.dtype], nat.ptr(weight),
+        nat.check(nat.lib().egnn_layer_norm_fwd(rows, cols, x.data_ptr(), x.stride(0), DTYPES[x.dtype], nat.ptr(weight),
                                                 nat.ptr(bias), nat.DTYPE_F32 if p is None else DTYPES[p.dtype], eps,
-                                                nat.ptr(y), nat.ptr(kept), nat.stream_ptr()), "egnn_layer_norm_fwd")
+                                                y.data_ptr(), nat.ptr(kept), nat.stream_ptr()), "egnn_layer_norm_fwd")
     return y, kept
+
+
+def _backward(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    rows, cols = x.shape
+    dy = _rows(dy)
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    pdt = weight.dtype if weight is not None else ctx.bias_dtype or torch.float32
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+    dw = db = ws = None
+    nbytes = 0
+    lib = nat.lib()
+    with nat.device_of(x):
+        if need_w:
+            dw = torch.empty_like(weight)
+        if need_b:
+            db = torch.empty(cols, dtype=pdt, device=x.device)
+        if need_w or need_b:
+            nbytes = lib.egnn_layer_norm_workspace_size(rows, cols)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        nat.check(lib.egnn_layer_norm_bwd(rows, cols, x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0),
+                                          DTYPES[x.dtype], nat.ptr(weight), DTYPES[pdt], stats.data_ptr(), nat.ptr(dx),
+                                          nat.ptr(dw), nat.ptr(db), nat.ptr(ws), nbytes, nat.stream_ptr()),
+                  "egnn_layer_norm_bwd")
+    return dx, dw, db, None
+
+
+_backward_once = torch.autograd.function.once_differentiable(_backward)
 
 
 class _LayerNormFn(torch.autograd.Function):
@@ -39,27 +67,9 @@ class _LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
-        rows, cols = x.shape
-        dy = _rows(dy)
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        pdt = weight.dtype if weight is not None else ctx.bias_dtype or torch.float32
-        dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty(cols, dtype=pdt, device=x.device) if need_w else None
-        db = torch.empty(cols, dtype=pdt, device=x.device) if need_b else None
-        lib = nat.lib()
-        with nat.device_of(x):
-            ws, ws_bytes = None, 0
-            if need_w or need_b:
-                ws_bytes = lib.egnn_layer_norm_workspace_size(rows, cols)
-                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-            nat.check(lib.egnn_layer_norm_bwd(rows, cols, nat.ptr(x), x.stride(0), nat.ptr(dy), dy.stride(0),
-                                              DTYPES[x.dtype], nat.ptr(weight), DTYPES[pdt], nat.ptr(stats),
-                                              nat.ptr(dx), nat.ptr(dw), nat.ptr(db), nat.ptr(ws), ws_bytes,
-                                              nat.stream_ptr()), "egnn_layer_norm_bwd")
-        return dx, dw, db, None
+        # grad mode is on only under create_graph, where a second derivative has to be refused
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def _rows(t):
@@ -77,31 +87,34 @@ def layer_norm(x: torch.Tensor, layer: nn.LayerNorm) -> torch.Tensor:
     """
     if not x.is_cuda:
         raise ValueError("layer_norm takes CUDA tensors (pymolecular_b200 has no CPU path)")
-    if x.dtype not in DTYPES:
-        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    shape = layer.normalized_shape
-    if len(shape) != 1 or x.dim() < 1 or x.shape[-1] != shape[0]:
-        raise ValueError(f"x must be (..., C) for a LayerNorm over its last axis alone, got {tuple(x.shape)} and "
+    dtype, size, shape = x.dtype, x.shape, layer.normalized_shape
+    if dtype not in DTYPES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {dtype}")
+    if len(shape) != 1 or not size or size[-1] != shape[0]:
+        raise ValueError(f"x must be (..., C) for a LayerNorm over its last axis alone, got {tuple(size)} and "
                          f"normalized_shape {tuple(shape)}")
     weight, bias = layer.weight, layer.bias
-    for name, p in (("weight", weight), ("bias", bias)):
+    needs_grad = x.requires_grad
+    for p in (weight, bias):
         if p is None:
             continue
         if p.device != x.device:
-            raise ValueError(f"the layer's {name} must be on {x.device}, got {p.device}")
-        if p.dtype not in (torch.float32, x.dtype) or (weight is not None and p.dtype != weight.dtype):
-            raise TypeError(f"the layer's {name} must be float32 or {x.dtype}, both parameters of one type, got {p.dtype}")
-    rows = x if x.dim() == 2 else x.reshape(-1, shape[0])
-    if rows.shape[0] > 1 or rows.stride(1) != 1:
+            raise ValueError(f"the layer's parameters must be on {x.device}, got {p.device}")
+        if p.dtype not in (torch.float32, dtype) or (weight is not None and p.dtype != weight.dtype):
+            raise TypeError(f"the layer's parameters must be float32 or {dtype}, both of one type, got {p.dtype}")
+        needs_grad = needs_grad or p.requires_grad
+    rows = x if len(size) == 2 else x.reshape(-1, shape[0])
+    if not rows.is_contiguous():
         rows = _rows(rows)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if needs_grad and torch.is_grad_enabled():
         y = _LayerNormFn.apply(rows, weight, bias, layer.eps)
     else:
-        y, _ = _forward(rows, weight, bias, layer.eps, False)
-    return y if x.dim() == 2 else y.view(x.shape)
+        y = _forward(rows, weight, bias, layer.eps, False)[0]
+    return y if len(size) == 2 else y.view(size)
 
 
 __all__ = ["layer_norm"]

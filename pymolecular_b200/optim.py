@@ -19,6 +19,8 @@ host, so a step with them can be captured (``graphs.GraphedStep``).
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import struct
 from typing import Iterable, List, Sequence, Tuple, Union
 
 import torch
@@ -31,14 +33,14 @@ STEPS = 5
 EPS = 1e-7
 
 
-def _options(steps, coefficients, eps):
-    a, b, c = coefficients
-    return nat.NsOptions(int(steps), 0, a, b, c, eps)
+@functools.lru_cache(maxsize=64)
+def _options(steps, a, b, c, eps):
+    return nat.NsOptions(steps, 0, a, b, c, eps)
 
 
 def _workspace(sizes: Sequence[int], device) -> Tuple[torch.Tensor, int]:
-    count = len(sizes) // 2
-    nbytes = nat.lib().egnn_orthogonalize_workspace_size(count, (C.c_int32 * len(sizes))(*sizes))
+    """sizes: rows, cols of each matrix in turn."""
+    nbytes = nat.lib().egnn_orthogonalize_workspace_size(len(sizes) // 2, struct.pack("%di" % len(sizes), *sizes))
     if not nbytes:
         raise ValueError("matrices have at most 16384 rows and columns, and the smaller side at most 1024")
     return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
@@ -50,48 +52,54 @@ def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = S
     its singular values driven towards 1 by `steps` Newton-Schulz products.
 
     float32, bfloat16 or float16 CUDA tensors of one device; the result has
-    each one's type and shape (dense), the products are as exact as
-    float32's.  Not differentiable: it treats `g` as data.
+    each one's type and shape (dense; the results of one size and type lie in
+    one allocation), the products are as exact as float32's.  Not
+    differentiable: it treats `g` as data.
     """
     if isinstance(g, torch.Tensor):
         if g.dim() < 2:
             raise ValueError("orthogonalize takes matrices")
-        if g.dim() == 2:
-            return orthogonalize([g], steps, coefficients, eps)[0]
-        flat = g.detach().reshape(-1, *g.shape[-2:])
-        out = torch.empty(flat.shape, dtype=g.dtype, device=g.device)
-        _orthogonalize(list(flat), list(out), steps, coefficients, eps)
-        return out.view(g.shape)
-    mats = [t.detach() for t in g]
-    out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in mats]
-    _orthogonalize(mats, out, steps, coefficients, eps)
-    return out
-
-
-def _orthogonalize(mats, out, steps, coefficients, eps):
-    if not mats:
-        return
-    device = mats[0].device
-    sizes, items = [], (nat.Matrix * len(mats))()
-    keep = []
-    for k, (t, o) in enumerate(zip(mats, out)):
-        if not t.is_cuda:
-            raise ValueError("orthogonalize takes CUDA tensors (pymolecular_b200 has no CPU path)")
-        if t.device != device:
-            raise ValueError("the matrices of a call must be on one device")
-        if t.dtype not in DTYPES:
-            raise TypeError(f"matrices must be float32, bfloat16 or float16, got {t.dtype}")
+        mats = g.detach().reshape(-1, *g.shape[-2:]).unbind(0)
+        if not mats:
+            return torch.empty_like(g, memory_format=torch.contiguous_format)
+    else:
+        mats = list(g)
+        if not mats:
+            return []
+    device = mats[0].get_device()
+    if device < 0:
+        raise ValueError("orthogonalize takes CUDA tensors (pymolecular_b200 has no CPU path)")
+    groups, sizes, copies = {}, [], []
+    for k, t in enumerate(mats):
         if t.dim() != 2:
             raise ValueError("orthogonalize takes matrices")
-        t = t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
-        keep.append(t)
-        rows, cols = t.shape
-        sizes += [rows, cols]
-        items[k] = nat.Matrix(nat.ptr(t), nat.ptr(o), t.stride(0), cols, rows, cols, DTYPES[t.dtype], 0)
+        if t.get_device() != device:
+            raise ValueError("the matrices of a call must be on one device")
+        size, dtype = t.shape, t.dtype
+        if dtype not in DTYPES:
+            raise TypeError(f"matrices must be float32, bfloat16 or float16, got {dtype}")
+        if not t.is_contiguous() and not (t.stride(1) == 1 and t.stride(0) >= size[1]):
+            t = t.contiguous()
+            copies.append(t)   # lives until the launch
+        sizes += size
+        groups.setdefault((size, dtype), []).append((k, t))
+    fields, out = [None] * len(mats), [None] * len(mats)
+    for (size, dtype), members in groups.items():
+        made = torch.empty((len(members), *size), dtype=dtype, device=device)
+        rows, cols = size
+        at, step, code = made.data_ptr(), rows * cols * made.element_size(), DTYPES[dtype]
+        for (k, t), o in zip(members, made.unbind(0)):
+            out[k] = o
+            fields[k] = (t.data_ptr(), at, t.stride(0), cols, rows | cols << 32, code)
+            at += step
     with nat.device_of(mats[0]):
         ws, nbytes = _workspace(sizes, device)
-        nat.check(nat.lib().egnn_orthogonalize(len(mats), items, C.byref(_options(steps, coefficients, eps)),
-                                               nat.ptr(ws), nbytes, nat.stream_ptr()), "egnn_orthogonalize")
+        items = struct.pack("%dQ" % (6 * len(mats)), *[v for f in fields for v in f])
+        nat.check(nat.lib().egnn_orthogonalize(len(mats), items, C.byref(_options(steps, *coefficients, eps)),
+                                               ws.data_ptr(), nbytes, nat.stream_ptr()), "egnn_orthogonalize")
+    if not isinstance(g, torch.Tensor):
+        return out
+    return made.view(g.shape)
 
 
 def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buffers: Sequence[torch.Tensor],
@@ -107,38 +115,52 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
         raise ValueError("muon_step takes one gradient and one momentum buffer for each parameter")
     if not params:
         return
-    if len({t.data_ptr() for t in (*params, *buffers) if t.numel()}) < sum(t.numel() > 0 for t in (*params, *buffers)):
+    if len({id(t) for t in (*params, *buffers)}) < 2 * len(params):
         raise ValueError("a parameter or momentum buffer is given twice")
-    device = params[0].device
+    device = params[0].get_device()
+    if device < 0:
+        raise ValueError("muon_step takes CUDA tensors (pymolecular_b200 has no CPU path)")
     on_device = isinstance(lr, torch.Tensor)
-    if on_device and (lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != device):
+    if on_device and (lr.numel() != 1 or lr.dtype != torch.float32 or lr.get_device() != device):
         raise ValueError("lr must be a number or one float32 on the parameters' device")
-    sizes, items, keep = [], (nat.MuonMatrix * len(params))(), []
+    f32 = torch.float32
+    sizes, fields, written, copies = [], [], [], []
     for k, (p, g, m) in enumerate(zip(params, grads, buffers)):
-        if not p.is_cuda:
-            raise ValueError("muon_step takes CUDA tensors (pymolecular_b200 has no CPU path)")
-        if p.dim() != 2 or p.shape != g.shape or p.shape != m.shape:
+        size = p.shape
+        if len(size) != 2 or g.shape != size or m.shape != size:
             raise ValueError(f"parameter {k}: a matrix and its gradient and momentum of the same shape are needed, got "
-                             f"{tuple(p.shape)}, {tuple(g.shape)}, {tuple(m.shape)}")
-        if p.device != device or g.device != device or m.device != device:
+                             f"{tuple(size)}, {tuple(g.shape)}, {tuple(m.shape)}")
+        if p.get_device() != device or g.get_device() != device or m.get_device() != device:
             raise ValueError("the tensors of a step must be on one device")
-        if p.dtype != torch.float32 or g.dtype != torch.float32 or m.dtype != torch.float32:
+        if p.dtype is not f32 or g.dtype is not f32 or m.dtype is not f32:
             raise TypeError("muon_step takes float32 parameters, gradients and momenta")
-        rows, cols = p.shape
-        for t in (p, m):
-            if rows * cols and (t.stride(1) != 1 and cols > 1 or t.stride(0) < cols and rows > 1):
-                raise ValueError("parameters and momenta must have dense rows (they are updated in place)")
-        g = g if g.stride(1) == 1 and g.stride(0) >= cols else g.contiguous()
-        keep.append(g)
-        sizes += [rows, cols]
-        items[k] = nat.MuonMatrix(nat.ptr(p), nat.ptr(g), nat.ptr(m), p.stride(0), g.stride(0), m.stride(0), rows, cols,
-                                  max(1.0, rows / max(cols, 1)) ** 0.5, 0)
-    options = nat.MuonOptions(_options(steps, coefficients, eps), momentum, weight_decay,
+        rows, cols = size
+        ldp = ldg = ldm = cols
+        if not (p.is_contiguous() and m.is_contiguous()):
+            ldp, ldm = p.stride(0), m.stride(0)
+            for t, ld in ((p, ldp), (m, ldm)):
+                if rows * cols and (t.stride(1) != 1 and cols > 1 or ld < cols and rows > 1):
+                    raise ValueError("parameters and momenta must have dense rows (they are updated in place)")
+        if not g.is_contiguous():
+            if g.stride(1) == 1 and g.stride(0) >= cols:
+                ldg = g.stride(0)
+            else:
+                g = g.contiguous()
+                copies.append(g)   # lives until the launch
+        sizes += size
+        pp, pm = p.data_ptr(), m.data_ptr()
+        if rows * cols:
+            written += (pp, pm)
+        fields += (pp, g.data_ptr(), pm, ldp, ldg, ldm, rows, cols, max(1.0, rows / max(cols, 1)) ** 0.5, 0)
+    if len(set(written)) < len(written):   # other tensors on the same memory
+        raise ValueError("a parameter or momentum buffer is given twice")
+    options = nat.MuonOptions(_options(steps, *coefficients, eps), momentum, weight_decay,
                               0.0 if on_device else lr, nat.ptr(lr) if on_device else None, int(nesterov), 0)
     with nat.device_of(params[0]):
         ws, nbytes = _workspace(sizes, device)
-        nat.check(nat.lib().egnn_muon_step(len(params), items, C.byref(options), nat.ptr(ws), nbytes, nat.stream_ptr()),
-                  "egnn_muon_step")
+        items = struct.pack("QQQqqqiifi" * len(params), *fields)
+        nat.check(nat.lib().egnn_muon_step(len(params), items, C.byref(options), ws.data_ptr(), nbytes,
+                                           nat.stream_ptr()), "egnn_muon_step")
     torch.autograd.graph.increment_version((*params, *buffers))
 
 
