@@ -1337,6 +1337,7 @@ extern "C" int egnn_device_status(void* stream) {
   n += node_tc_take_timeouts();
   n += rows_take_timeouts();
   n += ns_fused_take_timeouts();
+  n += ns_grid_take_timeouts();
   if (n != 0) {
     return fail(EGNN_ERR_CUDA, "%d tensor-core wait(s) timed out; results are invalid", n);
   }

@@ -12,6 +12,7 @@
 namespace egnn {
 
 constexpr int kNsItems = 64;   // matrices of one launch (kernel parameters)
+constexpr int kNsMaxSteps = 64;
 
 struct NsItem {
   const void* in;        // the matrix, or the gradient (float32) of a step
@@ -50,16 +51,6 @@ __device__ __forceinline__ T ns_from(float v) {
   else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
   else return __float2bfloat16_rn(v);
 }
-__device__ __forceinline__ float ns_load(const void* p, int dtype, int64_t i) {
-  if (dtype == EGNN_DTYPE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == EGNN_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ void ns_store(void* p, int dtype, int64_t i, float v) {
-  if (dtype == EGNN_DTYPE_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == EGNN_DTYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
 
 // M <- mu M + nu G, and U = mu M + nu G (Nesterov) or M from the moved M.
 __device__ __forceinline__ float ns_momentum(const NsScalars& q, float g, float m) { return fmaf(q.mu, m, q.nu * g); }
@@ -79,7 +70,12 @@ __device__ __forceinline__ void ns_rates(const NsItem& it, const NsScalars& q, f
 bool ns_fused_fits(int m, int n);
 // The matrices of the batch, one block each.
 int ns_fused(const NsBatch& b, const NsScalars& q, cudaStream_t s);
+// The matrices of the batch on the whole device, with workspace from `c`;
+// ns_grid_carve takes what one matrix needs.
+int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, cudaStream_t s);
+void ns_grid_carve(Carver& c, int rows, int cols);
 // Waits that ran out since the last call.
 int ns_fused_take_timeouts();
+int ns_grid_take_timeouts();
 
 }  // namespace egnn

@@ -17,8 +17,7 @@
 // for m > 32, 27 below.
 #include <atomic>
 
-#include "newton_schulz.cuh"
-#include "tc.cuh"
+#include "ns_tiles.cuh"
 
 namespace egnn {
 
@@ -27,6 +26,7 @@ __device__ int g_ns_fused_timeouts = 0;
 namespace {
 
 using namespace tc;
+using namespace ns;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
@@ -42,73 +42,6 @@ __host__ __device__ inline int tile_rows(int m) { return m <= 32 ? 32 : m <= 64 
 __host__ __device__ inline size_t smem_bytes(int m, int n) {
   const int R = tile_rows(m);
   return (size_t)((n + 63) / 64 + (m + 63) / 64) * R * 256 + (128 - R) * 128 + 1024;
-}
-
-// hi and lo tiles at (row, c0 .. c0 + 15) <- v[at .. at + 15].
-__device__ __forceinline__ void store_pairs16(char* hi, char* lo, int R, int row, int c0, const float* v) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float x = v[8 * j + 2 * k], y = v[8 * j + 2 * k + 1];
-      const __half2 p = __floats2half2_rn(x, y);
-      const float2 f = __half22float2(p);
-      const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-      h[k] = *reinterpret_cast<const uint32_t*>(&p);
-      l[k] = *reinterpret_cast<const uint32_t*>(&r);
-    }
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-  }
-}
-
-__device__ __forceinline__ void load_pairs32(const char* hi, const char* lo, int R, int row, int c0, float (&v)[32]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    const uint4 h = *reinterpret_cast<const uint4*>(hi + at), l = *reinterpret_cast<const uint4*>(lo + at);
-    const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&hh[k]));
-      const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&ll[k]));
-      v[8 * j + 2 * k] = p.x + r.x;
-      v[8 * j + 2 * k + 1] = p.y + r.y;
-    }
-  }
-}
-
-// The same places hold a float32's upper and lower 16 bits before the first
-// product and after the last.
-__device__ __forceinline__ void store_raw16(char* hi, char* lo, int R, int row, int c0, const float* v) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t x = __float_as_uint(v[8 * j + 2 * k]), y = __float_as_uint(v[8 * j + 2 * k + 1]);
-      h[k] = __byte_perm(x, y, 0x7632);
-      l[k] = __byte_perm(x, y, 0x5410);
-    }
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-  }
-}
-__device__ __forceinline__ void load_raw32(const char* hi, const char* lo, int R, int row, int c0, float (&v)[32]) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    const uint4 h = *reinterpret_cast<const uint4*>(hi + at), l = *reinterpret_cast<const uint4*>(lo + at);
-    const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[8 * j + 2 * k] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x5410));
-      v[8 * j + 2 * k + 1] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x7632));
-    }
-  }
 }
 
 // Issues D (+)= L R over the K-steps h, h + 2, h + 4, h + 6 (those below nk) of
@@ -134,47 +67,6 @@ __device__ __forceinline__ void issue3(uint32_t one, uint32_t d, uint64_t lh, ui
   issue<MN>(one, d, lh, rh, blk16, h, nk, idesc, 1);
 }
 
-// A warp's share of a matrix in global memory: units of 8 rows x 32 columns,
-// a column to a lane, so that an element costs few instructions besides its
-// access: the swizzle of row k of a unit is a constant of k.  In a turned
-// matrix the 8 rows are one 16-byte chunk of a tile row.
-struct Unit {
-  int id, per_row, r0, c;
-  __device__ __forceinline__ Unit(int cols) : id(threadIdx.x >> 5), per_row((cols + 31) >> 5) { place(); }
-  __device__ __forceinline__ void place() {
-    r0 = id / per_row * 8;
-    c = id % per_row * 32 + (threadIdx.x & 31);
-  }
-  __device__ __forceinline__ void next() {
-    id += kWarps;
-    place();
-  }
-};
-// Tile offset of element (r0 + k, c): chunk (k, in the low bits) of a tile whose column blocks are blk bytes.
-__device__ __forceinline__ uint32_t unit_row(const Unit& u, uint32_t blk, int k) {
-  return (u.c >> 6) * blk + ((u.r0 + k) << 7) + ((((u.c >> 3) & 7) ^ k) << 4) + ((u.c & 7) << 1);
-}
-__device__ __forceinline__ uint32_t unit_chunk(const Unit& u, uint32_t blk) {
-  return (u.r0 >> 6) * blk + (u.c << 7) + ((((u.r0 >> 3) & 7) ^ (u.c & 7)) << 4);
-}
-
-// The unit's 8 elements of this lane; zeros outside the matrix.
-template <typename T>
-__device__ __forceinline__ void unit_load(const T* p, int64_t ld, const Unit& u, int rows, int cols, float (&v)[8]) {
-  const int n = u.c < cols ? rows - u.r0 : 0;
-  p += u.r0 * ld + u.c;
-#pragma unroll
-  for (int k = 0; k < 8; ++k, p += ld) v[k] = k < n ? ns_float(*p) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void unit_store(T* p, int64_t ld, const Unit& u, int rows, int cols, const float (&v)[8]) {
-  const int n = u.c < cols ? rows - u.r0 : 0;
-  p += u.r0 * ld + u.c;
-#pragma unroll
-  for (int k = 0; k < 8; ++k, p += ld)
-    if (k < n) *p = ns_from<T>(v[k]);
-}
-
 // U into the tiles (raw); returns this thread's sum of squares, added in
 // float64: no overflow or underflow at any scale of the gradient.  The next
 // unit's loads are in flight while a unit is worked on.
@@ -189,7 +81,7 @@ __device__ __forceinline__ double take_in(const NsItem& it, const NsScalars& q, 
   const bool nesterov = q.nesterov;
   double ss = 0.0;
   float g[8], m[8];
-  Unit u(cols);
+  Unit u(cols, threadIdx.x >> 5, kWarps);
   if (u.r0 < rows) {
     unit_load(in, ld_in, u, rows, cols, g);
     if (MOM) unit_load(mom, ld_mom, u, rows, cols, m);
@@ -215,23 +107,11 @@ __device__ __forceinline__ double take_in(const NsItem& it, const NsScalars& q, 
     for (int k = 0; k < 8; ++k) ss = fma((double)g[k], (double)g[k], ss);
     if (u.c < cols) {   // rows past the matrix get the zeros that are there already
       if (turn) {
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t x = __float_as_uint(g[2 * k]), y = __float_as_uint(g[2 * k + 1]);
-          h[k] = __byte_perm(x, y, 0x7632);
-          l[k] = __byte_perm(x, y, 0x5410);
-        }
         const uint32_t o = unit_chunk(u, blk);
-        *reinterpret_cast<uint4*>(Xh + o) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(Xl + o) = make_uint4(l[0], l[1], l[2], l[3]);
+        store_chunk_raw(Xh + o, Xl + o, g);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t o = unit_row(u, blk, k), x = __float_as_uint(g[k]);
-          *reinterpret_cast<uint16_t*>(Xh + o) = (uint16_t)(x >> 16);
-          *reinterpret_cast<uint16_t*>(Xl + o) = (uint16_t)x;
-        }
+        for (int k = 0; k < 8; ++k) store_raw(Xh + unit_row(u, blk, k), Xl + unit_row(u, blk, k), g[k]);
       }
     }
     u = t;
@@ -254,7 +134,7 @@ __device__ __forceinline__ void give_out(const NsItem& it, const NsScalars& q, c
   float keep = 0.f, move = 0.f;
   if (MOM) ns_rates(it, q, keep, move);
   float w[8];
-  Unit u(cols);
+  Unit u(cols, threadIdx.x >> 5, kWarps);
   if (MOM && u.r0 < rows) unit_load(out, ld, u, rows, cols, w);
 #pragma unroll 1
   while (u.r0 < rows) {
@@ -265,20 +145,10 @@ __device__ __forceinline__ void give_out(const NsItem& it, const NsScalars& q, c
     if (u.c < cols) {
       if (turn) {
         const uint32_t o = unit_chunk(u, blk);
-        const uint4 h = *reinterpret_cast<const uint4*>(Xh + o), l = *reinterpret_cast<const uint4*>(Xl + o);
-        const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[2 * k] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x5410));
-          v[2 * k + 1] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x7632));
-        }
+        load_chunk_raw(Xh + o, Xl + o, v);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t o = unit_row(u, blk, k);
-          v[k] = __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(Xh + o) << 16 |
-                                 *reinterpret_cast<const uint16_t*>(Xl + o));
-        }
+        for (int k = 0; k < 8; ++k) v[k] = load_raw(Xh + unit_row(u, blk, k), Xl + unit_row(u, blk, k));
       }
       if (MOM)
 #pragma unroll
@@ -300,26 +170,12 @@ struct Barriers {
   uint64_t drained;
 };
 
-// Bounded wait, the same answer in the whole warp; false when it or another
-// warp's wait ran out.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-  bool ok = false;
-  for (uint32_t i = 0; i < (1u << 22) && !ok; ++i) {
-    ok = mbar_try_wait(bar, parity & 1u);
-    if (!ok && (i & 255u) == 255u && *gave_up) break;
-  }
-  ok = __all_sync(0xffffffffu, ok);
-  if (!ok) *gave_up = 1;
-  fence_after_sync();
-  return ok;
-}
 // This warp's tile writes and accumulator reads are done.
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   fence_proxy_async();
   fence_before_sync();
   __syncwarp();
-  if ((threadIdx.x & 31) == 0)
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // Warps 0 .. 15 take the matrix in, turn accumulators into operand tiles and
@@ -448,9 +304,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
     double ss = 0.0;
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) ss += red[k];
-    const double inv = 1.0 / (sqrt(ss) + q.eps);
-    // a power of two first, so that the rest of the scale is a float32 at any norm
-    const float pre = inv > 1.0 ? 0x1p64f : inv < 0x1p-64 ? 0x1p-64f : 1.f, f = (float)(inv / (double)pre);
+    float pre, f;
+    norm_scale(ss, q.eps, pre, f);
     // warp w owns tile rows 32 (w % 4) .. + 31, which are its accumulator lanes,
     // and of each group of four 32-column pieces the (w / 4)-th
     const int row = (warp & 3) * 32 + lane, piece = warp >> 2;

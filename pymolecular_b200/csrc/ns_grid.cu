@@ -1,0 +1,599 @@
+// Newton-Schulz iteration of matrices that a block's shared memory does not
+// hold: one cooperative launch whose blocks share out the matrices, each group
+// of blocks running all steps of its matrix on the tensor cores.
+//
+//   A = X X^T,  B = b A + c A A,  X <- a X + B X      (X m x n, m <= n)
+//
+// X (two buffers), A and B lie in the workspace as images: 128-row bands of
+// 64-column blocks, each block the 16 KB shared-memory form of an fp16 operand
+// (hi, and lo after all hi blocks), so that a bulk copy moves a block and the
+// same block serves as K-major and as MN-major operand.  Products are lo hi +
+// hi lo + hi hi as in the one-block kernel.  At these sizes images stay in L2.
+//
+// A block computes 128 x 128 tiles of its group's products: one warp streams
+// operands through a ring of three 64-column stages, one issues the products,
+// eight turn accumulators (two, used in turn) into images.  Blocks of a group
+// meet after each product at a counter in global memory; only the copies of the
+// next product wait for it.  The wait is bounded, and the launch is
+// cooperative, so all blocks are resident.
+//
+// An accumulator takes at most 768 terms: sums in tensor memory are rounded
+// towards zero at each instruction, so longer ones are added in float32
+// registers.
+#include <atomic>
+
+#include "ns_tiles.cuh"
+
+namespace egnn {
+
+__device__ int g_ns_grid_timeouts = 0;
+
+namespace {
+
+using namespace tc;
+using namespace ns;
+
+constexpr int kThreads = 320;          // copies, products, 8 warps of accumulator readers
+constexpr int kReaders = 8;
+constexpr int kStages = 3;
+constexpr int kBlk = 16384;            // bytes of a 128 x 64 block
+constexpr int kStageBytes = 4 * kBlk;  // hi and lo of both operands
+constexpr int kSegment = 12;           // 64-column chunks of one accumulator
+constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
+
+__host__ __device__ inline int up(int a, int b) { return (a + b - 1) / b; }
+
+struct Work {
+  char* x[2];            // images: hi blocks, then lo blocks
+  char *a, *b;
+  unsigned* counter;     // arrivals of the group's accumulator readers, for each product
+  double* partial;       // sums of squares of the parts of U
+};
+struct Grid {
+  NsItem it[kNsItems];
+  Work w[kNsItems];
+  int first[kNsItems + 1];   // first block of each matrix's group
+  int count;
+};
+constexpr int kParts = 32;   // blocks of a matrix in the norm
+
+struct Shape {
+  int m, n, m16, n16, bands, xc, ac;   // 128-row bands, 64-column blocks of X and of A
+  bool turn;
+  __host__ __device__ explicit Shape(const NsItem& it) {
+    turn = it.rows > it.cols;
+    m = turn ? it.cols : it.rows;
+    n = turn ? it.rows : it.cols;
+    m16 = (m + 15) & ~15;
+    n16 = (n + 15) & ~15;
+    bands = up(m, 128);
+    xc = up(n, 64);
+    ac = up(m, 64);
+  }
+  __host__ __device__ size_t x_bytes() const { return (size_t)bands * xc * kBlk; }   // of hi alone
+  __host__ __device__ size_t a_bytes() const { return (size_t)bands * ac * kBlk; }
+  // tiles of a product (0: A, 1: B, 2: X') and its 64-column chunks of K
+  __host__ __device__ int tile_cols(int mode) const { return mode == 2 ? up(n16, 128) : bands; }
+  __host__ __device__ int tiles(int mode) const { return bands * tile_cols(mode); }
+  __host__ __device__ int k16(int mode) const { return (mode == 0 ? n16 : m16) >> 4; }
+};
+
+// Image offset of the unit's element (r0 + k, c), or of its chunk where the matrix is turned.
+__device__ __forceinline__ size_t image_row(Unit u, int blocks, int k) {
+  const size_t band = (size_t)(u.r0 >> 7) * blocks * kBlk;
+  u.r0 &= 127;
+  return band + unit_row(u, kBlk, k);
+}
+__device__ __forceinline__ size_t image_chunk(Unit u, int blocks) {
+  const size_t band = (size_t)(u.c >> 7) * blocks * kBlk;
+  u.c &= 127;
+  return band + unit_chunk(u, kBlk);
+}
+
+// ---- U: momentum, and the sums of squares of kParts parts of each matrix ------
+__global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Grid g, const __grid_constant__ NsScalars q) {
+  pdl_enter();
+  __shared__ double red[8];
+  const NsItem& it = g.it[blockIdx.y];
+  const Work& w = g.w[blockIdx.y];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.x == 0)
+    for (int k = threadIdx.x; k < 3 * q.steps; k += 256) w.counter[k] = 0;
+  double ss = 0.0;
+  for (Unit u(it.cols, blockIdx.x * 8 + warp, kParts * 8); u.r0 < it.rows; u.next()) {
+    float v[8];
+    if (it.dtype == EGNN_DTYPE_F32) unit_load(static_cast<const float*>(it.in), it.ld_in, u, it.rows, it.cols, v);
+    else if (it.dtype == EGNN_DTYPE_BF16) unit_load(static_cast<const __nv_bfloat16*>(it.in), it.ld_in, u, it.rows, it.cols, v);
+    else unit_load(static_cast<const __half*>(it.in), it.ld_in, u, it.rows, it.cols, v);
+    if (it.mom) {
+      float mo[8];
+      unit_load(it.mom, it.ld_mom, u, it.rows, it.cols, mo);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        mo[k] = ns_momentum(q, v[k], mo[k]);
+        v[k] = ns_update(q, v[k], mo[k]);
+      }
+      unit_store(it.mom, it.ld_mom, u, it.rows, it.cols, mo);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ss = fma((double)v[k], (double)v[k], ss);
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+  if (lane == 0) red[warp] = ss;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int k = 1; k < 8; ++k) ss += red[k];
+  w.partial[blockIdx.x] = ss;
+}
+
+// ---- X0 as an image, zeros around the matrix ----------------------------------
+__global__ void __launch_bounds__(256) ns_image_kernel(const __grid_constant__ Grid g, const __grid_constant__ NsScalars q) {
+  pdl_enter();
+  const NsItem& it = g.it[blockIdx.y];
+  const Shape sh(it);
+  double ss = 0.0;
+  for (int k = 0; k < kParts; ++k) ss += g.w[blockIdx.y].partial[k];
+  float pre, f;
+  norm_scale(ss, q.eps, pre, f);
+  char* const hi = g.w[blockIdx.y].x[0];
+  char* const lo = hi + sh.x_bytes();
+  const int rows = sh.turn ? sh.xc * 64 : sh.bands * 128, cols = sh.turn ? sh.bands * 128 : sh.xc * 64;
+  for (Unit u(cols, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8); u.r0 < rows; u.next()) {
+    float v[8];
+    if (it.dtype == EGNN_DTYPE_F32) unit_load(static_cast<const float*>(it.in), it.ld_in, u, it.rows, it.cols, v);
+    else if (it.dtype == EGNN_DTYPE_BF16) unit_load(static_cast<const __nv_bfloat16*>(it.in), it.ld_in, u, it.rows, it.cols, v);
+    else unit_load(static_cast<const __half*>(it.in), it.ld_in, u, it.rows, it.cols, v);
+    if (it.mom) {
+      float mo[8];
+      unit_load(it.mom, it.ld_mom, u, it.rows, it.cols, mo);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = ns_update(q, v[k], mo[k]);
+    }
+    float h[8];   // as halves: hi in h, the rest in v
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] = v[k] * pre * f;
+      if (q.steps) {
+        v[k] *= q.sx;
+        h[k] = __half2float(__float2half_rn(v[k]));
+        v[k] -= h[k];
+      }
+    }
+    if (sh.turn) {
+      const size_t o = image_chunk(u, sh.xc);
+      if (q.steps) {
+        uint32_t a[4], b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const __half2 p = __floats2half2_rn(h[2 * k], h[2 * k + 1]), r = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+          a[k] = *reinterpret_cast<const uint32_t*>(&p);
+          b[k] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+        *reinterpret_cast<uint4*>(hi + o) = make_uint4(a[0], a[1], a[2], a[3]);
+        *reinterpret_cast<uint4*>(lo + o) = make_uint4(b[0], b[1], b[2], b[3]);
+      } else {
+        store_chunk_raw(hi + o, lo + o, v);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const size_t o = image_row(u, sh.xc, k);
+        if (q.steps) {
+          *reinterpret_cast<__half*>(hi + o) = __float2half_rn(h[k]);
+          *reinterpret_cast<__half*>(lo + o) = __float2half_rn(v[k]);
+        } else {
+          store_raw(hi + o, lo + o, v[k]);
+        }
+      }
+    }
+  }
+}
+
+// ---- the result out of the image, or the weight moved by it --------------------
+template <typename T>
+__device__ __forceinline__ void give(const NsItem& it, const NsScalars& q, const Shape& sh, const char* hi, const char* lo) {
+  T* const out = static_cast<T*>(it.out);
+  float keep = 0.f, move = 0.f;
+  if (it.mom) ns_rates(it, q, keep, move);
+  for (Unit u(it.cols, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8); u.r0 < it.rows; u.next()) {
+    float v[8], w[8];
+    if (u.c >= it.cols) continue;
+    if (it.mom) unit_load(out, it.ld_out, u, it.rows, it.cols, w);
+    if (sh.turn) {
+      const size_t o = image_chunk(u, sh.xc);
+      load_chunk_raw(hi + o, lo + o, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = load_raw(hi + image_row(u, sh.xc, k), lo + image_row(u, sh.xc, k));
+    }
+    if (it.mom)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = fmaf(move, v[k], keep * w[k]);
+    unit_store(out, it.ld_out, u, it.rows, it.cols, v);
+  }
+}
+__global__ void __launch_bounds__(256) ns_give_kernel(const __grid_constant__ Grid g, const __grid_constant__ NsScalars q) {
+  pdl_enter();
+  const NsItem& it = g.it[blockIdx.y];
+  const Shape sh(it);
+  const char* hi = g.w[blockIdx.y].x[q.steps & 1];
+  const char* lo = hi + sh.x_bytes();
+  if (it.dtype == EGNN_DTYPE_F32) give<float>(it, q, sh, hi, lo);
+  else if (it.dtype == EGNN_DTYPE_BF16) give<__nv_bfloat16>(it, q, sh, hi, lo);
+  else give<__half>(it, q, sh, hi, lo);
+}
+
+// ---- the steps ------------------------------------------------------------------
+struct Barriers {
+  uint64_t full[kStages], empty[kStages];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t drained;
+};
+
+// Generic writes to global memory <-> bulk copies of them.
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_constant__ Grid g,
+                                                              const __grid_constant__ NsScalars q) {
+  extern __shared__ char raw[];
+  __shared__ Barriers bar;
+  __shared__ uint32_t tmem_s;
+  __shared__ int gave_up_s;
+  const int lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  int item = 0;
+  while (item + 1 < g.count && g.first[item + 1] <= (int)blockIdx.x) ++item;
+  const Shape sh(g.it[item]);
+  const Work& w = g.w[item];
+  const int group = g.first[item + 1] - g.first[item], rank = blockIdx.x - g.first[item];
+  char* const ring = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  volatile int* const gave_up = &gave_up_s;
+
+  if (warp == 1) {
+    tmem_alloc(&tmem_s, 256);
+    if (lane == 0) {
+      gave_up_s = 0;
+      for (int k = 0; k < kStages; ++k) {
+        mbar_init(&bar.full[k], 1);
+        mbar_init(&bar.empty[k], 1);
+      }
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&bar.acc_full[k], 1);
+        mbar_init(&bar.acc_empty[k], kReaders);
+      }
+      mbar_init(&bar.drained, 1);
+      fence_mbar_init();
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_s;
+  const int phases = 3 * q.steps;
+  bool ok = true;
+
+  if (warp == 0) {
+    // ---- copies
+    int st = 0;
+    uint32_t ph = 1;   // a fresh barrier's previous phase counts as complete
+    int filled = 0;    // stages used so far, kStages at most
+#pragma unroll 1
+    for (int p = 0; p < phases && ok; ++p) {
+      const int mode = p % 3, cur = (p / 3) & 1;
+      if (p > 0) {   // every block of the group has written its tiles of the last product
+        bool here = false;
+        for (uint32_t i = 0; i < (1u << 23) && !here; ++i) {
+          here = load_acquire(w.counter + p - 1) == (unsigned)(group * kReaders);
+          if (!here && (i & 255u) == 255u && *gave_up) break;
+        }
+        here = __all_sync(0xffffffffu, here);
+        if (!here) {
+          *gave_up = 1;
+          ok = false;
+          break;
+        }
+        fence_proxy_async_all();
+      }
+      const char* Lh = mode == 0 ? w.x[cur] : mode == 1 ? w.a : w.b;
+      const char* Rh = mode == 1 ? w.a : w.x[cur];
+      const size_t lsize = mode == 0 ? sh.x_bytes() : sh.a_bytes(), rsize = mode == 1 ? sh.a_bytes() : sh.x_bytes();
+      const int lc = mode == 0 ? sh.xc : sh.ac;   // column blocks of L (and of a K-major R)
+      const int chunks = up(sh.k16(mode), 4), tn = sh.tile_cols(mode);
+#pragma unroll 1
+      for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
+        const int ti = t / tn, tj = t % tn;
+        const int rcols = mode == 2 ? min(2, sh.xc - 2 * tj) : 0;   // 64-column blocks of an MN-major R
+        const bool shared = mode != 2 && ti == tj;
+        const uint32_t bytes = 2 * kBlk + (mode == 2 ? rcols * kBlk : shared ? 0 : 2 * kBlk);
+#pragma unroll 1
+        for (int kc = 0; kc < chunks && ok; ++kc) {
+          if (!(ok = wait_bar(&bar.empty[st], ph, gave_up))) break;
+          if (lane == 0) {
+            char* const to = ring + st * kStageBytes;
+            const size_t l = (size_t)(ti * lc + kc) * kBlk;
+            mbar_expect_tx_bytes(&bar.full[st], bytes);
+            bulk_copy_g2s(to, Lh + l, kBlk, &bar.full[st]);
+            bulk_copy_g2s(to + kBlk, Lh + lsize + l, kBlk, &bar.full[st]);
+            if (mode == 2) {   // 64 rows of X: half of a block for each column block
+              for (int c = 0; c < rcols; ++c) {
+                const size_t r = (size_t)((kc >> 1) * sh.xc + 2 * tj + c) * kBlk + (kc & 1) * (kBlk / 2);
+                bulk_copy_g2s(to + 2 * kBlk + c * (kBlk / 2), Rh + r, kBlk / 2, &bar.full[st]);
+                bulk_copy_g2s(to + 3 * kBlk + c * (kBlk / 2), Rh + rsize + r, kBlk / 2, &bar.full[st]);
+              }
+            } else if (!shared) {
+              const size_t r = (size_t)(tj * lc + kc) * kBlk;
+              bulk_copy_g2s(to + 2 * kBlk, Rh + r, kBlk, &bar.full[st]);
+              bulk_copy_g2s(to + 3 * kBlk, Rh + rsize + r, kBlk, &bar.full[st]);
+            }
+          }
+          filled = min(filled + 1, kStages);
+          if (++st == kStages) {
+            st = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    }
+    // no copy may still be landing when the block ends: the products' warp has
+    // waited for every stage unless it gave up
+    if (*gave_up && filled) {
+      for (int k = 0; k < filled; ++k) {
+        st = st ? st - 1 : kStages - 1;
+        if (st == kStages - 1) ph ^= 1;
+        // stage st was last filled in the phase with parity ph ^ 1
+        bool in = false;
+        for (uint32_t i = 0; i < (1u << 16) && !in; ++i) in = mbar_try_wait(&bar.full[st], ph ^ 1u);
+      }
+    }
+  } else if (warp == 1) {
+    // ---- products
+    const uint32_t one = elect_one();
+    int st = 0, seg = 0;
+    uint32_t ph = 0;
+#pragma unroll 1
+    for (int p = 0; p < phases && ok; ++p) {
+      const int mode = p % 3, tn = sh.tile_cols(mode), k16 = sh.k16(mode), chunks = up(k16, 4);
+#pragma unroll 1
+      for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
+        const int ti = t / tn, tj = t % tn;
+        const bool shared = mode != 2 && ti == tj;
+        const uint32_t idesc = make_idesc_f16(128, min(128, (mode == 2 ? sh.n16 : sh.m16) - 128 * tj), 0, mode == 2);
+#pragma unroll 1
+        for (int kc = 0; kc < chunks && ok; ++kc) {
+          const bool start = kc % kSegment == 0;
+          // the accumulator's last user has been read
+          if (start && !(ok = wait_bar(&bar.acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, gave_up))) break;
+          if (!(ok = wait_bar(&bar.full[st], ph, gave_up))) break;
+          const uint32_t d = tmem + (seg & 1) * 128;
+          const uint32_t at = smem_u32(ring + st * kStageBytes), rt = shared ? at : at + 2 * kBlk;
+          const uint64_t lh = make_desc(at, 16, 1024), ll = make_desc(at + kBlk, 16, 1024);
+          const uint64_t rh = mode == 2 ? make_desc(rt, kBlk / 2, 1024) : make_desc(rt, 16, 1024);
+          const uint64_t rl = mode == 2 ? make_desc(rt + kBlk, kBlk / 2, 1024) : make_desc(rt + kBlk, 16, 1024);
+          const int nk = k16 - 4 * kc;
+          const uint32_t rstep = mode == 2 ? 128 : 2;
+#pragma unroll
+          for (int pr = 0; pr < 3; ++pr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < nk)
+                mma_f16_elected(one, d, (pr == 0 ? ll : lh) + 2 * j, (pr == 1 ? rl : rh) + rstep * j, idesc,
+                                !(start && pr == 0 && j == 0));
+          if (one) mma_commit(&bar.empty[st]);
+          if (++st == kStages) {
+            st = 0;
+            ph ^= 1;
+          }
+          if ((kc + 1) % kSegment == 0 || kc + 1 == chunks) {
+            if (one) mma_commit(&bar.acc_full[seg & 1]);
+            ++seg;
+          }
+        }
+      }
+    }
+    // nothing may be in flight when the tensor memory goes
+    if (one) mma_commit(&bar.drained);
+    wait_bar(&bar.drained, 0, gave_up);
+  } else {
+    // ---- accumulators into images: warp w reads the rows 32 (w % 4) .. + 31 and
+    // one half of the columns
+    const int row = (warp & 3) * 32 + lane, half = (warp - 2) >> 2;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const float fA = q.sa / (q.sx * q.sx);
+    const float fbA = q.b * q.sb / q.sa, fcAA = q.c * q.sb / (q.sa * q.sa);
+    const float fX = 1.f / q.sb, back = 1.f / q.sx;
+    int seg = 0;
+#pragma unroll 1
+    for (int p = 0; p < phases && ok; ++p) {
+      const int mode = p % 3, cur = (p / 3) & 1, tn = sh.tile_cols(mode), chunks = up(sh.k16(mode), 4);
+      const int blocks = mode == 2 ? sh.xc : sh.ac;
+      const size_t size = mode == 2 ? sh.x_bytes() : sh.a_bytes();
+      char* const dst = mode == 0 ? w.a : mode == 1 ? w.b : w.x[cur ^ 1];
+      const char* const old = mode == 1 ? w.a : w.x[cur];
+#pragma unroll 1
+      for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
+        const int ti = t / tn, tj = t % tn;
+        const int N = min(128, (mode == 2 ? sh.n16 : sh.m16) - 128 * tj);
+        float acc[2][32];
+#pragma unroll 1
+        for (int s0 = 0; s0 < chunks; s0 += kSegment, ++seg) {
+          if (!(ok = wait_bar(&bar.acc_full[seg & 1], (seg >> 1) & 1, gave_up))) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int c = half * 64 + i * 32;
+            if (c >= N) continue;
+            if (s0 == 0) {
+              tmem_ld32(tmem + (seg & 1) * 128 + lanes + c, acc[i]);
+            } else {
+              float v[32];
+              tmem_ld32(tmem + (seg & 1) * 128 + lanes + c, v);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) acc[i][k] += v[k];
+            }
+          }
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.acc_empty[seg & 1]);
+        }
+        if (!ok) break;
+        const size_t band = (size_t)ti * blocks * kBlk;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = half * 64 + i * 32;
+          if (c >= N) continue;
+          const int c0 = 128 * tj + c;
+          if (mode == 0) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[i][k] *= fA;
+          } else {
+            float o[32];   // this thread's own writes, or the first image
+            load_pairs32(old + band, old + size + band, 128, row, c0, o);
+            const float fo = mode == 1 ? fbA : q.a, fd = mode == 1 ? fcAA : fX;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[i][k] = fmaf(fo, o[k], fd * acc[i][k]);
+          }
+          if (p + 1 == phases) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[i][k] *= back;
+            store_raw16(dst + band, dst + size + band, 128, row, c0, acc[i]);
+            store_raw16(dst + band, dst + size + band, 128, row, c0 + 16, acc[i] + 16);
+          } else {
+            store_pairs16(dst + band, dst + size + band, 128, row, c0, acc[i]);
+            store_pairs16(dst + band, dst + size + band, 128, row, c0 + 16, acc[i] + 16);
+          }
+        }
+      }
+      if (!ok) break;
+      __threadfence();
+      fence_proxy_async_all();
+      __syncwarp();
+      if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(w.counter + p) : "memory");
+    }
+  }
+
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    if (lane == 0 && *gave_up) atomicAdd(&g_ns_grid_timeouts, 1);
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// The time of a matrix's step with a group of g blocks, in chunks of K.
+int step_time(const Shape& s, int g) {
+  int t = 0;
+  for (int mode = 0; mode < 3; ++mode) t += up(s.tiles(mode), g) * up(s.k16(mode), 4);
+  return t;
+}
+
+// Shares `blocks` out: again and again to the matrix that takes longest, as
+// many more as shorten its step.
+void share_out(Grid& g, int blocks) {
+  int size[kNsItems], time[kNsItems], left = blocks - g.count;
+  for (int i = 0; i < g.count; ++i) {
+    size[i] = 1;
+    time[i] = step_time(Shape(g.it[i]), 1);
+  }
+  while (left > 0) {
+    int worst = 0;
+    for (int i = 1; i < g.count; ++i)
+      if (time[i] > time[worst]) worst = i;
+    const Shape s(g.it[worst]);
+    const int most = std::min(size[worst] + left, std::max(s.tiles(0), s.tiles(2)));
+    int next = size[worst] + 1;
+    while (next <= most && step_time(s, next) >= time[worst]) ++next;
+    if (next > most) break;
+    left -= next - size[worst];
+    size[worst] = next;
+    time[worst] = step_time(s, next);
+  }
+  g.first[0] = 0;
+  for (int i = 0; i < g.count; ++i) g.first[i + 1] = g.first[i] + size[i];
+}
+
+Work carve_work(Carver& c, const Shape& s) {
+  Work w;
+  w.x[0] = c.take<char>(2 * s.x_bytes());
+  w.x[1] = c.take<char>(2 * s.x_bytes());
+  w.a = c.take<char>(2 * s.a_bytes());
+  w.b = c.take<char>(2 * s.a_bytes());
+  w.partial = c.take<double>(kParts);
+  w.counter = c.take<unsigned>(3 * kNsMaxSteps);
+  return w;
+}
+
+int run(Grid& g, const NsScalars& q, int blocks, cudaStream_t s) {
+  share_out(g, blocks);
+  int units = 1;
+  for (int i = 0; i < g.count; ++i) units = std::max(units, up(g.it[i].rows, 8) * up(g.it[i].cols, 32));
+  const dim3 grid(std::min(128, up(units, 16)), g.count);
+  TimerScope ts("newton_schulz", s);
+  EGNN_CHECK_CUDA(launch_pdl(ns_norm_kernel, dim3(kParts, g.count), dim3(256), 0, s, g, q));
+  EGNN_CHECK_LAUNCH();
+  EGNN_CHECK_CUDA(launch_pdl(ns_image_kernel, grid, dim3(256), 0, s, g, q));
+  EGNN_CHECK_LAUNCH();
+  if (q.steps) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(g.first[g.count]);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    EGNN_CHECK_CUDA(cudaLaunchKernelEx(&cfg, ns_grid_kernel, (const Grid&)g, q));
+    EGNN_CHECK_LAUNCH();
+  }
+  EGNN_CHECK_CUDA(launch_pdl(ns_give_kernel, grid, dim3(256), 0, s, g, q));
+  EGNN_CHECK_LAUNCH();
+  return EGNN_OK;
+}
+
+}  // namespace
+
+void ns_grid_carve(Carver& c, int rows, int cols) {
+  NsItem it = {};
+  it.rows = rows;
+  it.cols = cols;
+  carve_work(c, Shape(it));
+}
+
+int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  const uint64_t bit = device_bit();
+  if (!(ready.load() & bit)) {
+    EGNN_CHECK_CUDA(cudaFuncSetAttribute(ns_grid_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    ready.fetch_or(bit);
+  }
+  const int blocks = num_sms_current();
+  Grid g;
+  g.count = 0;
+  for (int i = 0; i < b.count; ++i) {
+    g.it[g.count] = b.it[i];
+    g.w[g.count] = carve_work(c, Shape(b.it[i]));
+    if (++g.count == std::min(kNsItems, blocks) || i + 1 == b.count) {
+      EGNN_TRY(run(g, q, blocks, s));
+      g.count = 0;
+    }
+  }
+  return EGNN_OK;
+}
+
+int ns_grid_take_timeouts() {
+  int n = 0;
+  if (cudaMemcpyFromSymbol(&n, g_ns_grid_timeouts, sizeof(int)) != cudaSuccess) return 0;
+  if (n) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_ns_grid_timeouts, &zero, sizeof(int));
+  }
+  return n;
+}
+
+}  // namespace egnn
