@@ -3,12 +3,11 @@
 //   A = X X^T,  B = b A + c A A,  X <- a X + B X      (X m x n, m <= n)
 //
 // Every product takes float32-like operands as pairs of fp16 tiles, v = hi + lo
-// with hi = fp16(v), lo = fp16(v - hi): 22 bits, against float32's 24.  The
-// three products lo hi, hi lo, hi hi accumulate in that order into one float32
-// accumulator in tensor memory, so that the small terms go in while the sum is
-// small; lo lo (2^-22 of the result) is left out.  Measured error against
-// float64 at 128 x 257: see the table of the design notes; float32 products
-// give the same.
+// with hi = fp16(v), lo = fp16(v - hi): 22 bits, against float32's 24.  lo lo
+// (2^-22 of the result) is left out.  Sums in tensor memory are rounded towards
+// zero at every instruction, by the size of the sum so far: lo hi + hi lo goes
+// into an accumulator of its own, or in before hi hi, so that only one
+// instruction per 16 terms costs a rounding of the full sum.
 //
 // X (hi, lo) and A, then B, (hi, lo) stay in shared memory through all steps:
 // global memory sees the matrix once on the way in and once on the way out.
@@ -58,15 +57,6 @@ __device__ __forceinline__ void issue(uint32_t one, uint32_t d, uint64_t l, uint
       accumulate = 1;
     }
 }
-// lo hi + hi lo + hi hi, in this order.
-template <bool MN>
-__device__ __forceinline__ void issue3(uint32_t one, uint32_t d, uint64_t lh, uint64_t ll, uint64_t rh, uint64_t rl,
-                                       uint32_t blk16, int h, int nk, uint32_t idesc, uint32_t accumulate) {
-  issue<MN>(one, d, ll, rh, blk16, h, nk, idesc, accumulate);
-  issue<MN>(one, d, lh, rl, blk16, h, nk, idesc, 1);
-  issue<MN>(one, d, lh, rh, blk16, h, nk, idesc, 1);
-}
-
 // U into the tiles (raw); returns this thread's sum of squares, added in
 // float64: no overflow or underflow at any scale of the gradient.  The next
 // unit's loads are in flight while a unit is worked on.
@@ -238,7 +228,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = tmem_s;
-  const uint32_t tA = tmem, tAA = tmem + kSlotCols;   // the slots 0 and 1, which hold X' only after B is made
+  // A and A A with their small terms apart: in the slots, which hold X' only after B is made
+  const uint32_t tA = tmem, tAA = tmem + kSlotCols, tAAx = tmem + 2 * kSlotCols, tAx = tmem + 3 * kSlotCols;
 
   if (warp == kWarps) {
     const uint32_t one = elect_one();
@@ -251,8 +242,8 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
     bool ok = true;
 #pragma unroll 1
     for (int step = 0; step < q.steps && ok; ++step) {
-      // a slot used more than once: its last X' columns have to be read before A goes there
-      for (int k = kSlots; k < chunks && ok; ++k)
+      // slot 3, and slots used more than once: their X' columns have to be read before A goes there
+      for (int k = kSlots - 1; k < chunks && ok; ++k)
         ok = wait_bar(&bar.x_ready[k][0], step, gave_up) && wait_bar(&bar.x_ready[k][1], step, gave_up);
 #pragma unroll 1
       for (int k = 0; k < chunks && ok; ++k)
@@ -260,14 +251,18 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
         for (int h = 0; h < 2 && ok; ++h) {
           if (!(ok = wait_bar(&bar.x_ready[k][h], step, gave_up))) break;
           const uint32_t o = 2 * k * blk16;
-          issue3<false>(one, tA, xh + o, xl + o, xh + o, xl + o, blk16, h, nk - 8 * k, idesc_m, k | h);
+          issue<false>(one, tAx, xl + o, xh + o, blk16, h, nk - 8 * k, idesc_m, k | h);
+          issue<false>(one, tAx, xh + o, xl + o, blk16, h, nk - 8 * k, idesc_m, 1);
+          issue<false>(one, tA, xh + o, xh + o, blk16, h, nk - 8 * k, idesc_m, k | h);
         }
       if (!ok) break;
       if (one) mma_commit(&bar.a_done);
 #pragma unroll 1
       for (int h = 0; h < 2 && ok; ++h) {
         if (!(ok = wait_bar(&bar.a_ready[h], step, gave_up))) break;
-        issue3<false>(one, tAA, ah, al, ah, al, blk16, h, mk, idesc_m, h);
+        issue<false>(one, tAAx, al, ah, blk16, h, mk, idesc_m, h);
+        issue<false>(one, tAAx, ah, al, blk16, h, mk, idesc_m, 1);
+        issue<false>(one, tAA, ah, ah, blk16, h, mk, idesc_m, h);
       }
       if (!ok) break;
       if (one) mma_commit(&bar.aa_done);
@@ -286,14 +281,16 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
                 !(ok = wait_bar(&bar.x_ready[k - kSlots][0], step + 1, gave_up) &&
                        wait_bar(&bar.x_ready[k - kSlots][1], step + 1, gave_up)))
               break;
-            const uint32_t o = 2 * k * blk16;
-            issue3<true>(one, tmem + (k - k0) * kSlotCols, ah, al, xh_mn + o, xl_mn + o, blk16, h, mk,
-                         make_idesc_f16(128, min(kSlotCols, n16 - k * kSlotCols), 0, 1), h);
-            if (h == 1 || mk == 1) {
+            const uint32_t o = 2 * k * blk16, d = tmem + (k - k0) * kSlotCols;
+            const uint32_t idesc = make_idesc_f16(128, min(kSlotCols, n16 - k * kSlotCols), 0, 1);
+            issue<true>(one, d, al, xh_mn + o, blk16, h, mk, idesc, h);
+            issue<true>(one, d, ah, xl_mn + o, blk16, h, mk, idesc, 1);
+            if (h == 1) {
+              issue<true>(one, d, ah, xh_mn + o, blk16, 0, mk, idesc, 1);
+              issue<true>(one, d, ah, xh_mn + o, blk16, 1, mk, idesc, 1);
               if (one) mma_commit(&bar.slot_done[k - k0]);
             }
           }
-          if (mk == 1) break;
         }
       }
     }
@@ -335,7 +332,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
     }
 
     const float fA = q.sa / (q.sx * q.sx);                    // accumulator -> A scaled
-    const float fbA = q.b * q.sb / (q.sx * q.sx), fcAA = q.c * q.sb / (q.sa * q.sa);
+    const float fbA = q.b * q.sb / q.sa, fcAA = q.c * q.sb / (q.sa * q.sa);
     const float fX = 1.f / q.sb, back = 1.f / q.sx;
     const bool a_here = rows_here && piece * 32 < m16;
     bool ok = true;
@@ -345,8 +342,9 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
       if (!(ok = wait_bar(&bar.a_done, step, gave_up))) break;
       if (a_here) {
         tmem_ld32(tA + lanes + piece * 32, v);
+        tmem_ld32(tAx + lanes + piece * 32, w);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] *= fA;
+        for (int k = 0; k < 32; ++k) v[k] = (v[k] + w[k]) * fA;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -355,10 +353,13 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
       }
       if (!(ok = wait_bar(&bar.aa_done, step, gave_up))) break;
       if (a_here) {
-        tmem_ld32(tA + lanes + piece * 32, v);
-        tmem_ld32(tAA + lanes + piece * 32, w);
+        load_pairs32(Ah, Al, R, row, piece * 32, w);   // this thread's own
+        tmem_ld32(tAA + lanes + piece * 32, v);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = fmaf(fbA, v[k], fcAA * w[k]);
+        for (int k = 0; k < 32; ++k) w[k] = fmaf(fbA, w[k], fcAA * v[k]);
+        tmem_ld32(tAAx + lanes + piece * 32, v);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = fmaf(fcAA, v[k], w[k]);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {

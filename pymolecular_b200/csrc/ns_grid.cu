@@ -17,9 +17,10 @@
 // next product wait for it.  The wait is bounded, and the launch is
 // cooperative, so all blocks are resident.
 //
-// An accumulator takes at most 768 terms: sums in tensor memory are rounded
-// towards zero at each instruction, so longer ones are added in float32
-// registers.
+// Sums in tensor memory are rounded towards zero at every instruction, by the
+// size of the sum so far.  So lo hi + hi lo has an accumulator of its own, and
+// an accumulator takes at most 128 terms, in 8 instructions; the pieces are
+// added in float32 registers.
 #include <atomic>
 
 #include "ns_tiles.cuh"
@@ -38,7 +39,7 @@ constexpr int kReaders = 8;
 constexpr int kStages = 3;
 constexpr int kBlk = 16384;            // bytes of a 128 x 64 block
 constexpr int kStageBytes = 4 * kBlk;  // hi and lo of both operands
-constexpr int kSegment = 12;           // 64-column chunks of one accumulator
+constexpr int kSegment = 2;            // 64-column chunks of one accumulator
 constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
 
 __host__ __device__ inline int up(int a, int b) { return (a + b - 1) / b; }
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   volatile int* const gave_up = &gave_up_s;
 
   if (warp == 1) {
-    tmem_alloc(&tmem_s, 256);
+    tmem_alloc(&tmem_s, 512);
     if (lane == 0) {
       gave_up_s = 0;
       for (int k = 0; k < kStages; ++k) {
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           // the accumulator's last user has been read
           if (start && !(ok = wait_bar(&bar.acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, gave_up))) break;
           if (!(ok = wait_bar(&bar.full[st], ph, gave_up))) break;
-          const uint32_t d = tmem + (seg & 1) * 128;
+          const uint32_t d = tmem + (seg & 1) * 256;   // hi hi, and the small terms 128 columns further
           const uint32_t at = smem_u32(ring + st * kStageBytes), rt = shared ? at : at + 2 * kBlk;
           const uint64_t lh = make_desc(at, 16, 1024), ll = make_desc(at + kBlk, 16, 1024);
           const uint64_t rh = mode == 2 ? make_desc(rt, kBlk / 2, 1024) : make_desc(rt, 16, 1024);
@@ -382,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (j < nk)
-                mma_f16_elected(one, d, (pr == 0 ? ll : lh) + 2 * j, (pr == 1 ? rl : rh) + rstep * j, idesc,
-                                !(start && pr == 0 && j == 0));
+                mma_f16_elected(one, pr == 2 ? d : d + 128, (pr == 0 ? ll : lh) + 2 * j, (pr == 1 ? rl : rh) + rstep * j,
+                                idesc, !(start && pr != 1 && j == 0));
           if (one) mma_commit(&bar.empty[st]);
           if (++st == kStages) {
             st = 0;
@@ -427,14 +428,18 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           for (int i = 0; i < 2; ++i) {
             const int c = half * 64 + i * 32;
             if (c >= N) continue;
+            float v[32];
+            tmem_ld32(tmem + (seg & 1) * 256 + 128 + lanes + c, v);
             if (s0 == 0) {
-              tmem_ld32(tmem + (seg & 1) * 128 + lanes + c, acc[i]);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) acc[i][k] = v[k];
             } else {
-              float v[32];
-              tmem_ld32(tmem + (seg & 1) * 128 + lanes + c, v);
 #pragma unroll
               for (int k = 0; k < 32; ++k) acc[i][k] += v[k];
             }
+            tmem_ld32(tmem + (seg & 1) * 256 + lanes + c, v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) acc[i][k] += v[k];
           }
           fence_before_sync();
           __syncwarp();
@@ -480,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   __syncthreads();
   if (warp == 1) {
     if (lane == 0 && *gave_up) atomicAdd(&g_ns_grid_timeouts, 1);
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 512);
   }
 }
 
