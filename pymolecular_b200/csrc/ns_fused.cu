@@ -29,8 +29,8 @@ using namespace ns;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kSlots = 4, kSlotCols = 128;   // X' accumulators in tensor memory
-constexpr int kMaxChunks = 16;               // of 128 columns of X: at most 27 column blocks fit
+constexpr int kSlots = 3, kSlotCols = 128;   // X' accumulators in tensor memory; B comes after them
+constexpr int kMaxChunks = 8;                // of 128 columns of X
 constexpr int kSmemMax = 232448 - 1024;      // a block's shared memory less the static part
 
 // Rows of a tile: all column blocks are `rows` x 128 bytes.
@@ -44,22 +44,54 @@ __host__ __device__ inline size_t smem_bytes(int m, int n) {
 }
 
 // Issues D (+)= L R over the K-steps h, h + 2, h + 4, h + 6 (those below nk) of
-// 128 columns of L.  L is K-major from descriptor l, R K-major too or MN-major
-// from r; blk16 is a column block in descriptor units.
-template <bool MN>
+// 128 columns of L, both K-major from their descriptors; blk16 is a column
+// block in descriptor units.
 __device__ __forceinline__ void issue(uint32_t one, uint32_t d, uint64_t l, uint64_t r, uint32_t blk16, int h, int nk,
                                       uint32_t idesc, uint32_t accumulate) {
 #pragma unroll
   for (int p = 0; p < 4; ++p)
     if (2 * p + h < nk) {
-      const uint32_t k_major = (p >> 1) * blk16 + (p & 1) * 4 + h * 2;
-      mma_f16_elected(one, d, l + k_major, r + (MN ? (2 * p + h) * 128 : k_major), idesc, accumulate);
+      const uint32_t o = (p >> 1) * blk16 + (p & 1) * 4 + h * 2;
+      mma_f16_elected(one, d, l + o, r + o, idesc, accumulate);
       accumulate = 1;
     }
 }
+// The same with L in tensor memory and R MN-major.
+__device__ __forceinline__ void issue_mn(uint32_t one, uint32_t d, uint32_t l, uint64_t r, int h, int nk, uint32_t idesc,
+                                         uint32_t accumulate) {
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    if (2 * p + h < nk) {
+      mma_f16_ts_elected(one, d, l + (2 * p + h) * 8, r + (2 * p + h) * 128, idesc, accumulate);
+      accumulate = 1;
+    }
+}
+
+// The units of a matrix two at a time, the next two's loads in flight while
+// two are worked on: load(unit, slot) and work(unit, slot).
+template <class Load, class Work>
+__device__ __forceinline__ void units(int rows, int cols, const Load& load, const Work& work) {
+  Unit u[2] = {Unit(cols, threadIdx.x >> 5, kWarps), Unit(cols, (threadIdx.x >> 5) + kWarps, kWarps)};
+  if (u[0].r0 < rows) load(u[0], 0);
+  if (u[1].r0 < rows) load(u[1], 1);
+#pragma unroll 1
+  while (u[0].r0 < rows) {
+    Unit t[2] = {u[0], u[1]};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t[i].id += kWarps;
+      t[i].next();
+      if (t[i].r0 < rows) load(t[i], 2 + i);
+    }
+    work(u[0], 0);
+    if (u[1].r0 < rows) work(u[1], 1);
+    u[0] = t[0];
+    u[1] = t[1];
+  }
+}
+
 // U into the tiles (raw); returns this thread's sum of squares, added in
-// float64: no overflow or underflow at any scale of the gradient.  The next
-// unit's loads are in flight while a unit is worked on.
+// float64: no overflow or underflow at any scale of the gradient.
 template <typename T, bool MOM>
 __device__ __forceinline__ double take_in(const NsItem& it, const NsScalars& q, char* Xh, char* Xl, uint32_t blk,
                                           bool turn) {
@@ -70,47 +102,32 @@ __device__ __forceinline__ double take_in(const NsItem& it, const NsScalars& q, 
   const float mu = q.mu, nu = q.nu;
   const bool nesterov = q.nesterov;
   double ss = 0.0;
-  float g[8], m[8];
-  Unit u(cols, threadIdx.x >> 5, kWarps);
-  if (u.r0 < rows) {
-    unit_load(in, ld_in, u, rows, cols, g);
-    if (MOM) unit_load(mom, ld_mom, u, rows, cols, m);
-  }
-#pragma unroll 1
-  while (u.r0 < rows) {
-    float g2[8], m2[8];
-    Unit t = u;
-    t.next();
-    if (t.r0 < rows) {
-      unit_load(in, ld_in, t, rows, cols, g2);
-      if (MOM) unit_load(mom, ld_mom, t, rows, cols, m2);
-    }
-    if (MOM) {
+  float g[4][8], m[4][8];
+  units(
+      rows, cols,
+      [&](const Unit& u, int i) {
+        unit_load(in, ld_in, u, rows, cols, g[i]);
+        if (MOM) unit_load(mom, ld_mom, u, rows, cols, m[i]);
+      },
+      [&](const Unit& u, int i) {
+        if (MOM) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        m[k] = fmaf(mu, m[k], nu * g[k]);
-        g[k] = nesterov ? fmaf(mu, m[k], nu * g[k]) : m[k];
-      }
-      unit_store(mom, ld_mom, u, rows, cols, m);
-    }
+          for (int k = 0; k < 8; ++k) {
+            m[i][k] = fmaf(mu, m[i][k], nu * g[i][k]);
+            g[i][k] = nesterov ? fmaf(mu, m[i][k], nu * g[i][k]) : m[i][k];
+          }
+          unit_store(mom, ld_mom, u, rows, cols, m[i]);
+        }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fma((double)g[k], (double)g[k], ss);
-    if (u.c < cols) {   // rows past the matrix get the zeros that are there already
-      if (turn) {
-        const uint32_t o = unit_chunk(u, blk);
-        store_chunk_raw(Xh + o, Xl + o, g);
-      } else {
+        for (int k = 0; k < 8; ++k) ss = fma((double)g[i][k], (double)g[i][k], ss);
+        // rows past the matrix get the zeros that are there already
+        if (u.c < cols) unit_to_raw(Xh, Xl, blk, turn, u, g[i]);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) store_raw(Xh + unit_row(u, blk, k), Xl + unit_row(u, blk, k), g[k]);
-      }
-    }
-    u = t;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      g[k] = g2[k];
-      if (MOM) m[k] = m2[k];
-    }
-  }
+        for (int k = 0; k < 8; ++k) {
+          g[i][k] = g[2 + i][k];
+          if (MOM) m[i][k] = m[2 + i][k];
+        }
+      });
   return ss;
 }
 
@@ -123,33 +140,25 @@ __device__ __forceinline__ void give_out(const NsItem& it, const NsScalars& q, c
   const int64_t ld = it.ld_out;
   float keep = 0.f, move = 0.f;
   if (MOM) ns_rates(it, q, keep, move);
-  float w[8];
-  Unit u(cols, threadIdx.x >> 5, kWarps);
-  if (MOM && u.r0 < rows) unit_load(out, ld, u, rows, cols, w);
-#pragma unroll 1
-  while (u.r0 < rows) {
-    float w2[8], v[8];
-    Unit t = u;
-    t.next();
-    if (MOM && t.r0 < rows) unit_load(out, ld, t, rows, cols, w2);
-    if (u.c < cols) {
-      if (turn) {
-        const uint32_t o = unit_chunk(u, blk);
-        load_chunk_raw(Xh + o, Xl + o, v);
-      } else {
+  float w[4][8];
+  units(
+      rows, cols,
+      [&](const Unit& u, int i) {
+        if (MOM) unit_load(out, ld, u, rows, cols, w[i]);
+      },
+      [&](const Unit& u, int i) {
+        if (u.c < cols) {
+          float v[8];
+          unit_from_raw(Xh, Xl, blk, turn, u, v);
+          if (MOM)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = load_raw(Xh + unit_row(u, blk, k), Xl + unit_row(u, blk, k));
-      }
-      if (MOM)
+            for (int k = 0; k < 8; ++k) v[k] = fmaf(move, v[k], keep * w[i][k]);
+          unit_store(out, ld, u, rows, cols, v);
+        }
+        if (MOM)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = fmaf(move, v[k], keep * w[k]);
-      unit_store(out, ld, u, rows, cols, v);
-    }
-    u = t;
-    if (MOM)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = w2[k];
-  }
+          for (int k = 0; k < 8; ++k) w[i][k] = w[2 + i][k];
+      });
 }
 
 struct Barriers {
@@ -228,8 +237,16 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = tmem_s;
-  // A and A A with their small terms apart: in the slots, which hold X' only after B is made
+  // The slots hold X' only after B is made, so A and A A, their small terms apart, go there.  Long sums
+  // are spread over three accumulators.
+  const int sums = chunks > kSlots ? kSlots : 1;
   const uint32_t tA = tmem, tAA = tmem + kSlotCols, tAAx = tmem + 2 * kSlotCols, tAx = tmem + 3 * kSlotCols;
+  const uint32_t tB = tAx, tBl = tB + 64;   // hi and lo of B
+  // which use of its slot X' columns k are in a step
+  auto slot_use = [&](int step, int k) {
+    const int slot = k % kSlots;
+    return step * ((chunks - slot + kSlots - 1) / kSlots) + k / kSlots;
+  };
 
   if (warp == kWarps) {
     const uint32_t one = elect_one();
@@ -242,27 +259,29 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
     bool ok = true;
 #pragma unroll 1
     for (int step = 0; step < q.steps && ok; ++step) {
-      // slot 3, and slots used more than once: their X' columns have to be read before A goes there
-      for (int k = kSlots - 1; k < chunks && ok; ++k)
+      // slots used more than once: their last X' columns have to be read before A goes there
+      for (int k = kSlots; k < chunks && ok; ++k)
         ok = wait_bar(&bar.x_ready[k][0], step, gave_up) && wait_bar(&bar.x_ready[k][1], step, gave_up);
+      // B has been read by the last of the products
+      if (step > 0 && ok) ok = wait_bar(&bar.slot_done[(chunks - 1) % kSlots], slot_use(step - 1, chunks - 1), gave_up);
 #pragma unroll 1
       for (int k = 0; k < chunks && ok; ++k)
 #pragma unroll 1
         for (int h = 0; h < 2 && ok; ++h) {
           if (!(ok = wait_bar(&bar.x_ready[k][h], step, gave_up))) break;
-          const uint32_t o = 2 * k * blk16;
-          issue<false>(one, tAx, xl + o, xh + o, blk16, h, nk - 8 * k, idesc_m, k | h);
-          issue<false>(one, tAx, xh + o, xl + o, blk16, h, nk - 8 * k, idesc_m, 1);
-          issue<false>(one, tA, xh + o, xh + o, blk16, h, nk - 8 * k, idesc_m, k | h);
+          const uint32_t o = 2 * k * blk16, d = tmem + (k % sums) * kSlotCols;
+          issue(one, tAx, xl + o, xh + o, blk16, h, nk - 8 * k, idesc_m, k | h);
+          issue(one, tAx, xh + o, xl + o, blk16, h, nk - 8 * k, idesc_m, 1);
+          issue(one, d, xh + o, xh + o, blk16, h, nk - 8 * k, idesc_m, k >= sums || h);
         }
       if (!ok) break;
       if (one) mma_commit(&bar.a_done);
 #pragma unroll 1
       for (int h = 0; h < 2 && ok; ++h) {
         if (!(ok = wait_bar(&bar.a_ready[h], step, gave_up))) break;
-        issue<false>(one, tAAx, al, ah, blk16, h, mk, idesc_m, h);
-        issue<false>(one, tAAx, ah, al, blk16, h, mk, idesc_m, 1);
-        issue<false>(one, tAA, ah, ah, blk16, h, mk, idesc_m, h);
+        issue(one, tAAx, al, ah, blk16, h, mk, idesc_m, h);
+        issue(one, tAAx, ah, al, blk16, h, mk, idesc_m, 1);
+        issue(one, tAA, ah, ah, blk16, h, mk, idesc_m, h);
       }
       if (!ok) break;
       if (one) mma_commit(&bar.aa_done);
@@ -283,11 +302,11 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
               break;
             const uint32_t o = 2 * k * blk16, d = tmem + (k - k0) * kSlotCols;
             const uint32_t idesc = make_idesc_f16(128, min(kSlotCols, n16 - k * kSlotCols), 0, 1);
-            issue<true>(one, d, al, xh_mn + o, blk16, h, mk, idesc, h);
-            issue<true>(one, d, ah, xl_mn + o, blk16, h, mk, idesc, 1);
+            issue_mn(one, d, tBl, xh_mn + o, h, mk, idesc, h);
+            issue_mn(one, d, tB, xl_mn + o, h, mk, idesc, 1);
             if (h == 1) {
-              issue<true>(one, d, ah, xh_mn + o, blk16, 0, mk, idesc, 1);
-              issue<true>(one, d, ah, xh_mn + o, blk16, 1, mk, idesc, 1);
+              issue_mn(one, d, tB, xh_mn + o, 0, mk, idesc, 1);
+              issue_mn(one, d, tB, xh_mn + o, 1, mk, idesc, 1);
               if (one) mma_commit(&bar.slot_done[k - k0]);
             }
           }
@@ -344,7 +363,14 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
         tmem_ld32(tA + lanes + piece * 32, v);
         tmem_ld32(tAx + lanes + piece * 32, w);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = (v[k] + w[k]) * fA;
+        for (int k = 0; k < 32; ++k) v[k] += w[k];
+        for (int j = 1; j < sums; ++j) {
+          tmem_ld32(tmem + j * kSlotCols + lanes + piece * 32, w);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] += w[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= fA;
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -363,13 +389,19 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (a_here) store_pairs16(Ah, Al, R, row, piece * 32 + 16 * h, v + 16 * h);
+        if (a_here) {
+          uint32_t hw[8], lw[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) split2(v[16 * h + 2 * k], v[16 * h + 2 * k + 1], hw[k], lw[k]);
+          tmem_st8u(tB + lanes + piece * 16 + 8 * h, hw);
+          tmem_st8u(tBl + lanes + piece * 16 + 8 * h, lw);
+        }
         arrive(&bar.b_ready[h]);
       }
 #pragma unroll 1
       for (int k = 0; k < chunks; ++k) {
-        const int slot = k % kSlots, uses = (chunks - slot + kSlots - 1) / kSlots;   // of this slot in a step
-        if (!(ok = wait_bar(&bar.slot_done[slot], step * uses + k / kSlots, gave_up))) break;
+        const int slot = k % kSlots;
+        if (!(ok = wait_bar(&bar.slot_done[slot], slot_use(step, k), gave_up))) break;
         const int c0 = k * kSlotCols + piece * 32;
         const bool here = rows_here && c0 < n16;
         if (here) {

@@ -79,16 +79,12 @@ struct Shape {
   __host__ __device__ int k16(int mode) const { return (mode == 0 ? n16 : m16) >> 4; }
 };
 
-// Image offset of the unit's element (r0 + k, c), or of its chunk where the matrix is turned.
-__device__ __forceinline__ size_t image_row(Unit u, int blocks, int k) {
-  const size_t band = (size_t)(u.r0 >> 7) * blocks * kBlk;
-  u.r0 &= 127;
-  return band + unit_row(u, kBlk, k);
-}
-__device__ __forceinline__ size_t image_chunk(Unit u, int blocks) {
-  const size_t band = (size_t)(u.c >> 7) * blocks * kBlk;
-  u.c &= 127;
-  return band + unit_chunk(u, kBlk);
+// The band of an image that a unit lies in; its row there becomes a tile row.
+__device__ __forceinline__ size_t to_band(Unit& u, int blocks, bool turn) {
+  int& r = turn ? u.c : u.r0;
+  const size_t band = (size_t)(r >> 7) * blocks * kBlk;
+  r &= 127;
+  return band;
 }
 
 // ---- U: momentum, and the sums of squares of kParts parts of each matrix ------
@@ -151,42 +147,16 @@ __global__ void __launch_bounds__(256) ns_image_kernel(const __grid_constant__ G
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = ns_update(q, v[k], mo[k]);
     }
-    float h[8];   // as halves: hi in h, the rest in v
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      v[k] = v[k] * pre * f;
-      if (q.steps) {
-        v[k] *= q.sx;
-        h[k] = __half2float(__float2half_rn(v[k]));
-        v[k] -= h[k];
-      }
-    }
-    if (sh.turn) {
-      const size_t o = image_chunk(u, sh.xc);
-      if (q.steps) {
-        uint32_t a[4], b[4];
+    for (int k = 0; k < 8; ++k) v[k] = v[k] * pre * f;
+    Unit t = u;
+    const size_t band = to_band(t, sh.xc, sh.turn);
+    if (q.steps) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const __half2 p = __floats2half2_rn(h[2 * k], h[2 * k + 1]), r = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-          a[k] = *reinterpret_cast<const uint32_t*>(&p);
-          b[k] = *reinterpret_cast<const uint32_t*>(&r);
-        }
-        *reinterpret_cast<uint4*>(hi + o) = make_uint4(a[0], a[1], a[2], a[3]);
-        *reinterpret_cast<uint4*>(lo + o) = make_uint4(b[0], b[1], b[2], b[3]);
-      } else {
-        store_chunk_raw(hi + o, lo + o, v);
-      }
+      for (int k = 0; k < 8; ++k) v[k] *= q.sx;
+      unit_to_pairs(hi + band, lo + band, 128, sh.turn, t, v);
     } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const size_t o = image_row(u, sh.xc, k);
-        if (q.steps) {
-          *reinterpret_cast<__half*>(hi + o) = __float2half_rn(h[k]);
-          *reinterpret_cast<__half*>(lo + o) = __float2half_rn(v[k]);
-        } else {
-          store_raw(hi + o, lo + o, v[k]);
-        }
-      }
+      unit_to_raw(hi + band, lo + band, kBlk, sh.turn, t, v);
     }
   }
 }
@@ -201,13 +171,9 @@ __device__ __forceinline__ void give(const NsItem& it, const NsScalars& q, const
     float v[8], w[8];
     if (u.c >= it.cols) continue;
     if (it.mom) unit_load(out, it.ld_out, u, it.rows, it.cols, w);
-    if (sh.turn) {
-      const size_t o = image_chunk(u, sh.xc);
-      load_chunk_raw(hi + o, lo + o, v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = load_raw(hi + image_row(u, sh.xc, k), lo + image_row(u, sh.xc, k));
-    }
+    Unit t = u;
+    const size_t band = to_band(t, sh.xc, sh.turn);
+    unit_from_raw(hi + band, lo + band, kBlk, sh.turn, t, v);
     if (it.mom)
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = fmaf(move, v[k], keep * w[k]);

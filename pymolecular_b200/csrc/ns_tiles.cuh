@@ -10,20 +10,22 @@ namespace ns {
 
 using tc::sw128_offset;
 
-// hi and lo tiles at (row, c0 .. c0 + 15) <- v[at .. at + 15].
+// x, y as fp16 pairs hi + lo, x in the lower half of the words.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& h, uint32_t& l) {
+  const __half2 p = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(p);
+  const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+  h = *reinterpret_cast<const uint32_t*>(&p);
+  l = *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// hi and lo tiles at (row, c0 .. c0 + 15) <- v.
 __device__ __forceinline__ void store_pairs16(char* hi, char* lo, int R, int row, int c0, const float* v) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     uint32_t h[4], l[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float x = v[8 * j + 2 * k], y = v[8 * j + 2 * k + 1];
-      const __half2 p = __floats2half2_rn(x, y);
-      const float2 f = __half22float2(p);
-      const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
-      h[k] = *reinterpret_cast<const uint32_t*>(&p);
-      l[k] = *reinterpret_cast<const uint32_t*>(&r);
-    }
+    for (int k = 0; k < 4; ++k) split2(v[8 * j + 2 * k], v[8 * j + 2 * k + 1], h[k], l[k]);
     const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
     *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -46,62 +48,94 @@ __device__ __forceinline__ void load_pairs32(const char* hi, const char* lo, int
   }
 }
 
-// The same places hold a float32's upper and lower 16 bits before the first
-// product and after the last.
+// Before the first product and after the last, the bytes of 32 columns of a
+// row in both tiles hold them as float32: columns 0 .. 15 where the hi halves
+// are, 16 .. 31 where the lo halves are.  Offset of column c in its tile:
+__device__ __forceinline__ uint32_t raw_offset(int row, int c, uint32_t blk) {
+  return (c >> 6) * blk + (row << 7) + ((((c >> 3 & 4) | (c >> 2 & 3)) ^ (row & 7)) << 4) + ((c & 3) << 2);
+}
 __device__ __forceinline__ void store_raw16(char* hi, char* lo, int R, int row, int c0, const float* v) {
+  char* const t = c0 & 16 ? lo : hi;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t x = __float_as_uint(v[8 * j + 2 * k]), y = __float_as_uint(v[8 * j + 2 * k + 1]);
-      h[k] = __byte_perm(x, y, 0x7632);
-      l[k] = __byte_perm(x, y, 0x5410);
-    }
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-  }
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<float4*>(t + raw_offset(row, c0 + 4 * j, R * 128)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
 }
 __device__ __forceinline__ void load_raw32(const char* hi, const char* lo, int R, int row, int c0, float (&v)[32]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    const uint4 h = *reinterpret_cast<const uint4*>(hi + at), l = *reinterpret_cast<const uint4*>(lo + at);
-    const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[8 * j + 2 * k] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x5410));
-      v[8 * j + 2 * k + 1] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x7632));
-    }
+  for (int j = 0; j < 8; ++j) {
+    const float4 x = *reinterpret_cast<const float4*>((j & 4 ? lo : hi) + raw_offset(row, c0 + 4 * j, R * 128));
+    v[4 * j] = x.x;
+    v[4 * j + 1] = x.y;
+    v[4 * j + 2] = x.z;
+    v[4 * j + 3] = x.w;
   }
 }
 
 // A warp's share of a matrix in global memory: units of 8 rows x 32 columns,
 // a column to a lane, so that an element costs few instructions besides its
-// access: the swizzle of row k of a unit is a constant of k.  In a turned
-// matrix the 8 rows are one 16-byte chunk of a tile row.
+// access: the swizzle of row k of a unit is a constant of k.  Two units share
+// 64 columns, 16 of each 32 to a unit: those lie in one tile and in all its
+// banks.  In a turned matrix the 8 rows are two chunks of a tile row.
 struct Unit {
   int id, per_row, stride, r0, c;
   __device__ __forceinline__ Unit(int cols, int first, int stride_)
-      : id(first), per_row((cols + 31) >> 5), stride(stride_) {
+      : id(first), per_row((cols + 63) / 64 * 2), stride(stride_) {
     place();
   }
   __device__ __forceinline__ void place() {
+    const int lane = threadIdx.x & 31, j = id % per_row;
     r0 = id / per_row * 8;
-    c = id % per_row * 32 + (threadIdx.x & 31);
+    c = (j >> 1) * 64 + (lane & 16) * 2 + (j & 1) * 16 + (lane & 15);
   }
   __device__ __forceinline__ void next() {
     id += stride;
     place();
   }
 };
-// Tile offset of element (r0 + k, c): chunk (k, in the low bits) of a tile whose column blocks are blk bytes.
-__device__ __forceinline__ uint32_t unit_row(const Unit& u, uint32_t blk, int k) {
-  return (u.c >> 6) * blk + ((u.r0 + k) << 7) + ((((u.c >> 3) & 7) ^ k) << 4) + ((u.c & 7) << 1);
+// The raw elements (r0 .. r0 + 7, c) of a tile, or (c, r0 .. r0 + 7) of a turned one.
+__device__ __forceinline__ void unit_to_raw(char* hi, char* lo, uint32_t blk, bool turn, const Unit& u, const float (&v)[8]) {
+  if (turn) {
+    char* const t = u.r0 & 16 ? lo : hi;
+    *reinterpret_cast<float4*>(t + raw_offset(u.c, u.r0, blk)) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(t + raw_offset(u.c, u.r0 + 4, blk)) = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    char* const t = u.c & 16 ? lo : hi;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) *reinterpret_cast<float*>(t + raw_offset(u.r0 + k, u.c, blk)) = v[k];
+  }
 }
-__device__ __forceinline__ uint32_t unit_chunk(const Unit& u, uint32_t blk) {
-  return (u.r0 >> 6) * blk + (u.c << 7) + ((((u.r0 >> 3) & 7) ^ (u.c & 7)) << 4);
+__device__ __forceinline__ void unit_from_raw(const char* hi, const char* lo, uint32_t blk, bool turn, const Unit& u,
+                                              float (&v)[8]) {
+  if (turn) {
+    const char* const t = u.r0 & 16 ? lo : hi;
+    const float4 x = *reinterpret_cast<const float4*>(t + raw_offset(u.c, u.r0, blk));
+    const float4 y = *reinterpret_cast<const float4*>(t + raw_offset(u.c, u.r0 + 4, blk));
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  } else {
+    const char* const t = u.c & 16 ? lo : hi;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const float*>(t + raw_offset(u.r0 + k, u.c, blk));
+  }
+}
+// The same of pairs.
+__device__ __forceinline__ void unit_to_pairs(char* hi, char* lo, int R, bool turn, const Unit& u, const float (&v)[8]) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) split2(v[2 * k], v[2 * k + 1], h[k], l[k]);
+  if (turn) {
+    const uint32_t at = sw128_offset(u.c, u.r0, R);
+    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t at = sw128_offset(u.r0 + k, u.c, R);
+      *reinterpret_cast<uint16_t*>(hi + at) = (uint16_t)(h[k >> 1] >> (k & 1) * 16);
+      *reinterpret_cast<uint16_t*>(lo + at) = (uint16_t)(l[k >> 1] >> (k & 1) * 16);
+    }
+  }
 }
 
 // The unit's 8 elements of this lane; zeros outside the matrix.
@@ -119,37 +153,6 @@ __device__ __forceinline__ void unit_store(T* p, int64_t ld, const Unit& u, int 
 #pragma unroll
   for (int k = 0; k < 8; ++k, p += ld)
     if (k < n) *p = ns_from<T>(v[k]);
-}
-
-// 8 float32 <-> one chunk of a tile row (raw halves).
-__device__ __forceinline__ void store_chunk_raw(char* hi, char* lo, const float (&v)[8]) {
-  uint32_t h[4], l[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t x = __float_as_uint(v[2 * k]), y = __float_as_uint(v[2 * k + 1]);
-    h[k] = __byte_perm(x, y, 0x7632);
-    l[k] = __byte_perm(x, y, 0x5410);
-  }
-  *reinterpret_cast<uint4*>(hi) = make_uint4(h[0], h[1], h[2], h[3]);
-  *reinterpret_cast<uint4*>(lo) = make_uint4(l[0], l[1], l[2], l[3]);
-}
-__device__ __forceinline__ void load_chunk_raw(const char* hi, const char* lo, float (&v)[8]) {
-  const uint4 h = *reinterpret_cast<const uint4*>(hi), l = *reinterpret_cast<const uint4*>(lo);
-  const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    v[2 * k] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x5410));
-    v[2 * k + 1] = __uint_as_float(__byte_perm(ll[k], hh[k], 0x7632));
-  }
-}
-__device__ __forceinline__ void store_raw(char* hi, char* lo, float v) {
-  const uint32_t x = __float_as_uint(v);
-  *reinterpret_cast<uint16_t*>(hi) = (uint16_t)(x >> 16);
-  *reinterpret_cast<uint16_t*>(lo) = (uint16_t)x;
-}
-__device__ __forceinline__ float load_raw(const char* hi, const char* lo) {
-  return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(hi) << 16 |
-                         *reinterpret_cast<const uint16_t*>(lo));
 }
 
 // The scale 1 / (norm + eps) as pre * f: a power of two first, so that f is a
