@@ -34,7 +34,7 @@ struct NsBatch {
 struct NsScalars {
   float a, b, c;
   double eps;
-  float sx, sa, sb;         // scales of X, A and B
+  float sx, sa, sb;         // scales of X, A and b A + c A A
   float mu, nu;             // nu = 1 - mu
   double decay, lr;
   const float* lr_device;
@@ -63,6 +63,15 @@ __device__ __forceinline__ void ns_rates(const NsItem& it, const NsScalars& q, f
   const double lr = q.lr_device ? (double)*q.lr_device : q.lr;
   keep = (float)(1.0 - lr * q.decay);
   move = (float)(-lr * it.gain);
+}
+
+// A sum in tensor memory is rounded towards zero at each of its L instructions.
+// On average one loses half a unit in the last place of the sum so far, which
+// is 2^-23 / (4 ln 2) of it, and sums so far average (L + 1) / 2L of the whole:
+// the mean loss, relative to the sum, that the readers add back.  What is left
+// is its scatter.
+__host__ __device__ inline float ns_mean_loss(int instructions) {
+  return 0x1p-23f * 0.3607f * 0.5f * (float)(instructions + 1);
 }
 
 // Whether one block's shared memory holds the whole iteration of an m x n

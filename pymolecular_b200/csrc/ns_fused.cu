@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
     const float fA = q.sa / (q.sx * q.sx);                    // accumulator -> A scaled
     const float fbA = q.b * q.sb / q.sa, fcAA = q.c * q.sb / (q.sa * q.sa);
     const float fX = 1.f / q.sb, back = 1.f / q.sx;
+    const float loss_n = ns_mean_loss((n16 >> 4) / sums), loss_m = ns_mean_loss(m16 >> 4);
     const bool a_here = rows_here && piece * 32 < m16;
     bool ok = true;
 #pragma unroll 1
@@ -361,14 +362,14 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
       if (!(ok = wait_bar(&bar.a_done, step, gave_up))) break;
       if (a_here) {
         tmem_ld32(tA + lanes + piece * 32, v);
-        tmem_ld32(tAx + lanes + piece * 32, w);
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] += w[k];
         for (int j = 1; j < sums; ++j) {
           tmem_ld32(tmem + j * kSlotCols + lanes + piece * 32, w);
 #pragma unroll
           for (int k = 0; k < 32; ++k) v[k] += w[k];
         }
+        tmem_ld32(tAx + lanes + piece * 32, w);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = fmaf(v[k], loss_n, v[k]) + w[k];
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] *= fA;
       }
@@ -382,7 +383,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
         load_pairs32(Ah, Al, R, row, piece * 32, w);   // this thread's own
         tmem_ld32(tAA + lanes + piece * 32, v);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) w[k] = fmaf(fbA, w[k], fcAA * v[k]);
+        for (int k = 0; k < 32; ++k) w[k] = fmaf(fbA, w[k], fcAA * fmaf(v[k], loss_m, v[k]));
         tmem_ld32(tAAx + lanes + piece * 32, v);
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = fmaf(fcAA, v[k], w[k]);
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
           tmem_ld32(tmem + lanes + slot * kSlotCols + piece * 32, v);
           load_pairs32(Xh, Xl, R, row, c0, w);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(q.a, w[j], fX * v[j]);
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(q.a, w[j], fX * fmaf(v[j], loss_m, v[j]));
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {

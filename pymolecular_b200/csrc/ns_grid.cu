@@ -11,11 +11,16 @@
 // hi lo + hi hi as in the one-block kernel.  At these sizes images stay in L2.
 //
 // A block computes 128 x 128 tiles of its group's products: one warp streams
-// operands through a ring of three 64-column stages, one issues the products,
-// eight turn accumulators (two, used in turn) into images.  Blocks of a group
-// meet after each product at a counter in global memory; only the copies of the
-// next product wait for it.  The wait is bounded, and the launch is
+// operands through a ring of 64-column stages, one issues the products, sixteen
+// turn accumulators (two, used in turn) into blocks of an image, which leave
+// through shared memory as bulk copies: 16-byte stores to global memory and the
+// fence behind them took 8,300 cycles a tile, these copies REPLACE_ME.  Blocks of a
+// group meet after each product at a counter in global memory; only the copies
+// of the next product wait for it.  The wait is bounded, and the launch is
 // cooperative, so all blocks are resident.
+//
+// What bounds it: at one to three tiles a product the chain of copy latency,
+// products, accumulator reads and the meeting, not the tensor cores.
 //
 // Sums in tensor memory are rounded towards zero at every instruction, by the
 // size of the sum so far.  So lo hi + hi lo has an accumulator of its own, and
@@ -34,20 +39,20 @@ namespace {
 using namespace tc;
 using namespace ns;
 
-constexpr int kThreads = 320;          // copies, products, 8 warps of accumulator readers
-constexpr int kReaders = 8;
-constexpr int kStages = 3;
+constexpr int kReaders = 16;           // warps that read accumulators
+constexpr int kThreads = 64 + 32 * kReaders;   // and one of copies, one of products
+constexpr int kMaxStages = 8;
 constexpr int kBlk = 16384;            // bytes of a 128 x 64 block
-constexpr int kStageBytes = 4 * kBlk;  // hi and lo of both operands
+constexpr int kRing = 12 * kBlk;
 constexpr int kSegment = 2;            // 64-column chunks of one accumulator
-constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024;
+constexpr size_t kSmem = kRing + 2 * kBlk + 1024;   // the ring, the blocks on their way out, alignment
 
 __host__ __device__ inline int up(int a, int b) { return (a + b - 1) / b; }
 
 struct Work {
   char* x[2];            // images: hi blocks, then lo blocks
   char *a, *b;
-  unsigned* counter;     // arrivals of the group's accumulator readers, for each product
+  unsigned* counter;     // arrivals of the group's blocks, for each product
   double* partial;       // sums of squares of the parts of U
 };
 struct Grid {
@@ -76,6 +81,16 @@ struct Shape {
   // tiles of a product (0: A, 1: B, 2: X') and its 64-column chunks of K
   __host__ __device__ int tile_cols(int mode) const { return mode == 2 ? up(n16, 128) : bands; }
   __host__ __device__ int tiles(int mode) const { return bands * tile_cols(mode); }
+  // rows of a band that hold anything (those a copy moves), and the ring's stages
+  __host__ __device__ int band_rows(int band) const { return m16 - 128 * band < 128 ? m16 - 128 * band : 128; }
+  __host__ __device__ int stage_bytes(int mode) const {
+    const int rows = band_rows(0) * 128;   // a block of the highest band
+    return 2 * rows + (mode == 2 ? 2 * kBlk : bands > 1 ? 2 * rows : 0);
+  }
+  __host__ __device__ int stages(int mode) const {
+    const int s = kRing / stage_bytes(mode);
+    return s < kMaxStages ? s : kMaxStages;
+  }
   __host__ __device__ int k16(int mode) const { return (mode == 0 ? n16 : m16) >> 4; }
 };
 
@@ -193,17 +208,30 @@ __global__ void __launch_bounds__(256) ns_give_kernel(const __grid_constant__ Gr
 
 // ---- the steps ------------------------------------------------------------------
 struct Barriers {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  uint64_t old_read[kMaxStages];         // the readers have taken A or X out of the stage
   uint64_t acc_full[2], acc_empty[2];
+  uint64_t written, out_free;            // the blocks on their way out
   uint64_t drained;
 };
 
-// Generic writes to global memory <-> bulk copies of them.
+// Generic accesses of global memory <-> bulk copies.
 __device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
   unsigned v;
   asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
+}
+__device__ __forceinline__ void bulk_copy_s2g(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+// B and X' add a multiple of the same tile of A or X to their product.  That
+// tile comes through the ring anyhow: as two chunks of L (A: columns 2 tj, 2 tj + 1)
+// or of R (X: rows of the band ti), from where the readers take it.
+__device__ __forceinline__ bool old_chunk(int mode, int ti, int tj, int kc) {
+  return mode != 0 && (kc >> 1) == (mode == 1 ? tj : ti);
 }
 
 __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_constant__ Grid g,
@@ -220,20 +248,24 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   const Work& w = g.w[item];
   const int group = g.first[item + 1] - g.first[item], rank = blockIdx.x - g.first[item];
   char* const ring = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  char* const out = ring + kRing;
   volatile int* const gave_up = &gave_up_s;
 
   if (warp == 1) {
     tmem_alloc(&tmem_s, 512);
     if (lane == 0) {
       gave_up_s = 0;
-      for (int k = 0; k < kStages; ++k) {
+      for (int k = 0; k < kMaxStages; ++k) {
         mbar_init(&bar.full[k], 1);
         mbar_init(&bar.empty[k], 1);
+        mbar_init(&bar.old_read[k], kReaders);
       }
       for (int k = 0; k < 2; ++k) {
         mbar_init(&bar.acc_full[k], 1);
         mbar_init(&bar.acc_empty[k], kReaders);
       }
+      mbar_init(&bar.written, kReaders);
+      mbar_init(&bar.out_free, 1);
       mbar_init(&bar.drained, 1);
       fence_mbar_init();
     }
@@ -246,17 +278,17 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   bool ok = true;
 
   if (warp == 0) {
-    // ---- copies
-    int st = 0;
-    uint32_t ph = 1;   // a fresh barrier's previous phase counts as complete
-    int filled = 0;    // stages used so far, kStages at most
+    // ---- copies.  Before a product's first copy all of the last one's are read
+    // (this block's own arrival says so), so the ring is cut anew for each.
+    uint32_t used = 0, parity = 0;   // bit k: stage k has been filled; the parity of its last filling
+    uint32_t old = 0, old_parity = 0;   // the same of its fillings with a chunk that the readers take from
 #pragma unroll 1
     for (int p = 0; p < phases && ok; ++p) {
       const int mode = p % 3, cur = (p / 3) & 1;
       if (p > 0) {   // every block of the group has written its tiles of the last product
         bool here = false;
         for (uint32_t i = 0; i < (1u << 23) && !here; ++i) {
-          here = load_acquire(w.counter + p - 1) == (unsigned)(group * kReaders);
+          here = load_acquire(w.counter + p - 1) == (unsigned)group;
           if (!here && (i & 255u) == 255u && *gave_up) break;
         }
         here = __all_sync(0xffffffffu, here);
@@ -272,60 +304,64 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
       const size_t lsize = mode == 0 ? sh.x_bytes() : sh.a_bytes(), rsize = mode == 1 ? sh.a_bytes() : sh.x_bytes();
       const int lc = mode == 0 ? sh.xc : sh.ac;   // column blocks of L (and of a K-major R)
       const int chunks = up(sh.k16(mode), 4), tn = sh.tile_cols(mode);
+      const int stages = sh.stages(mode), stage_bytes = sh.stage_bytes(mode), full_rows = sh.band_rows(0) * 128;
+      int st = 0;
 #pragma unroll 1
       for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
         const int ti = t / tn, tj = t % tn;
         const int rcols = mode == 2 ? min(2, sh.xc - 2 * tj) : 0;   // 64-column blocks of an MN-major R
         const bool shared = mode != 2 && ti == tj;
-        const uint32_t bytes = 2 * kBlk + (mode == 2 ? rcols * kBlk : shared ? 0 : 2 * kBlk);
+        const uint32_t lbytes = sh.band_rows(ti) * 128, rbytes = mode == 2 || shared ? 0 : sh.band_rows(tj) * 128;
+        const uint32_t bytes = 2 * lbytes + 2 * rbytes + rcols * kBlk;
 #pragma unroll 1
         for (int kc = 0; kc < chunks && ok; ++kc) {
-          if (!(ok = wait_bar(&bar.empty[st], ph, gave_up))) break;
+          if ((used >> st & 1u) && !(ok = wait_bar(&bar.empty[st], parity >> st & 1u, gave_up))) break;
+          if (old >> st & 1u) {
+            if (!(ok = wait_bar(&bar.old_read[st], old_parity >> st & 1u, gave_up))) break;
+            old &= ~(1u << st);
+            old_parity ^= 1u << st;
+          }
+          if (old_chunk(mode, ti, tj, kc)) old |= 1u << st;
+          if (used >> st & 1u) parity ^= 1u << st;
+          used |= 1u << st;
           if (lane == 0) {
-            char* const to = ring + st * kStageBytes;
+            char* const to = ring + st * stage_bytes;
             const size_t l = (size_t)(ti * lc + kc) * kBlk;
             mbar_expect_tx_bytes(&bar.full[st], bytes);
-            bulk_copy_g2s(to, Lh + l, kBlk, &bar.full[st]);
-            bulk_copy_g2s(to + kBlk, Lh + lsize + l, kBlk, &bar.full[st]);
+            bulk_copy_g2s(to, Lh + l, lbytes, &bar.full[st]);
+            bulk_copy_g2s(to + full_rows, Lh + lsize + l, lbytes, &bar.full[st]);
+            char* const rt = to + 2 * full_rows;
             if (mode == 2) {   // 64 rows of X: half of a block for each column block
               for (int c = 0; c < rcols; ++c) {
                 const size_t r = (size_t)((kc >> 1) * sh.xc + 2 * tj + c) * kBlk + (kc & 1) * (kBlk / 2);
-                bulk_copy_g2s(to + 2 * kBlk + c * (kBlk / 2), Rh + r, kBlk / 2, &bar.full[st]);
-                bulk_copy_g2s(to + 3 * kBlk + c * (kBlk / 2), Rh + rsize + r, kBlk / 2, &bar.full[st]);
+                bulk_copy_g2s(rt + c * (kBlk / 2), Rh + r, kBlk / 2, &bar.full[st]);
+                bulk_copy_g2s(rt + kBlk + c * (kBlk / 2), Rh + rsize + r, kBlk / 2, &bar.full[st]);
               }
             } else if (!shared) {
               const size_t r = (size_t)(tj * lc + kc) * kBlk;
-              bulk_copy_g2s(to + 2 * kBlk, Rh + r, kBlk, &bar.full[st]);
-              bulk_copy_g2s(to + 3 * kBlk, Rh + rsize + r, kBlk, &bar.full[st]);
+              bulk_copy_g2s(rt, Rh + r, rbytes, &bar.full[st]);
+              bulk_copy_g2s(rt + full_rows, Rh + rsize + r, rbytes, &bar.full[st]);
             }
           }
-          filled = min(filled + 1, kStages);
-          if (++st == kStages) {
-            st = 0;
-            ph ^= 1;
-          }
+          if (++st == stages) st = 0;
         }
       }
     }
-    // no copy may still be landing when the block ends: the products' warp has
-    // waited for every stage unless it gave up
-    if (*gave_up && filled) {
-      for (int k = 0; k < filled; ++k) {
-        st = st ? st - 1 : kStages - 1;
-        if (st == kStages - 1) ph ^= 1;
-        // stage st was last filled in the phase with parity ph ^ 1
-        bool in = false;
-        for (uint32_t i = 0; i < (1u << 16) && !in; ++i) in = mbar_try_wait(&bar.full[st], ph ^ 1u);
+    if (*gave_up)   // no copy may still be landing when the block ends
+      for (int k = 0; k < kMaxStages; ++k) {
+        bool in = !(used >> k & 1u);
+        for (uint32_t i = 0; i < (1u << 16) && !in; ++i) in = mbar_try_wait(&bar.full[k], parity >> k & 1u);
       }
-    }
   } else if (warp == 1) {
     // ---- products
     const uint32_t one = elect_one();
-    int st = 0, seg = 0;
-    uint32_t ph = 0;
+    int seg = 0;
+    uint32_t parity = 0;   // of each stage's next filling
 #pragma unroll 1
     for (int p = 0; p < phases && ok; ++p) {
       const int mode = p % 3, tn = sh.tile_cols(mode), k16 = sh.k16(mode), chunks = up(k16, 4);
+      const int stages = sh.stages(mode), stage_bytes = sh.stage_bytes(mode), full_rows = sh.band_rows(0) * 128;
+      int st = 0;
 #pragma unroll 1
       for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
         const int ti = t / tn, tj = t % tn;
@@ -336,12 +372,13 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           const bool start = kc % kSegment == 0;
           // the accumulator's last user has been read
           if (start && !(ok = wait_bar(&bar.acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, gave_up))) break;
-          if (!(ok = wait_bar(&bar.full[st], ph, gave_up))) break;
+          if (!(ok = wait_bar(&bar.full[st], parity >> st & 1u, gave_up))) break;
+          parity ^= 1u << st;
           const uint32_t d = tmem + (seg & 1) * 256;   // hi hi, and the small terms 128 columns further
-          const uint32_t at = smem_u32(ring + st * kStageBytes), rt = shared ? at : at + 2 * kBlk;
-          const uint64_t lh = make_desc(at, 16, 1024), ll = make_desc(at + kBlk, 16, 1024);
+          const uint32_t at = smem_u32(ring + st * stage_bytes), rt = shared ? at : at + 2 * full_rows;
+          const uint64_t lh = make_desc(at, 16, 1024), ll = make_desc(at + full_rows, 16, 1024);
           const uint64_t rh = mode == 2 ? make_desc(rt, kBlk / 2, 1024) : make_desc(rt, 16, 1024);
-          const uint64_t rl = mode == 2 ? make_desc(rt + kBlk, kBlk / 2, 1024) : make_desc(rt + kBlk, 16, 1024);
+          const uint64_t rl = mode == 2 ? make_desc(rt + kBlk, kBlk / 2, 1024) : make_desc(rt + full_rows, 16, 1024);
           const int nk = k16 - 4 * kc;
           const uint32_t rstep = mode == 2 ? 128 : 2;
 #pragma unroll
@@ -352,10 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
                 mma_f16_elected(one, pr == 2 ? d : d + 128, (pr == 0 ? ll : lh) + 2 * j, (pr == 1 ? rl : rh) + rstep * j,
                                 idesc, !(start && pr != 1 && j == 0));
           if (one) mma_commit(&bar.empty[st]);
-          if (++st == kStages) {
-            st = 0;
-            ph ^= 1;
-          }
+          if (++st == stages) st = 0;
           if ((kc + 1) % kSegment == 0 || kc + 1 == chunks) {
             if (one) mma_commit(&bar.acc_full[seg & 1]);
             ++seg;
@@ -367,84 +401,148 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     if (one) mma_commit(&bar.drained);
     wait_bar(&bar.drained, 0, gave_up);
   } else {
-    // ---- accumulators into images: warp w reads the rows 32 (w % 4) .. + 31 and
-    // one half of the columns
-    const int row = (warp & 3) * 32 + lane, half = (warp - 2) >> 2;
+    // ---- accumulators into images: warp w reads the rows 32 (w % 4) .. + 31 of
+    // one 32-column piece
+    const int row = (warp & 3) * 32 + lane, c = ((warp - 2) >> 2) * 32;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const float fA = q.sa / (q.sx * q.sx);
-    const float fbA = q.b * q.sb / q.sa, fcAA = q.c * q.sb / (q.sa * q.sa);
-    const float fX = 1.f / q.sb, back = 1.f / q.sx;
-    int seg = 0;
+    const float loss = ns_mean_loss(4 * kSegment);
+    int seg = 0, outs = 0, frees = 0;
+    uint32_t parity = 0;   // of each stage's next filling
 #pragma unroll 1
     for (int p = 0; p < phases && ok; ++p) {
       const int mode = p % 3, cur = (p / 3) & 1, tn = sh.tile_cols(mode), chunks = up(sh.k16(mode), 4);
       const int blocks = mode == 2 ? sh.xc : sh.ac;
       const size_t size = mode == 2 ? sh.x_bytes() : sh.a_bytes();
+      const int stages = sh.stages(mode), stage_bytes = sh.stage_bytes(mode), full_rows = sh.band_rows(0) * 128;
+      int st = 0;
       char* const dst = mode == 0 ? w.a : mode == 1 ? w.b : w.x[cur ^ 1];
-      const char* const old = mode == 1 ? w.a : w.x[cur];
+      const bool last = p + 1 == phases;   // X' itself, not scaled
+      // weights of the product and of the old tile
+      const float end = last ? 1.f / q.sx : 1.f;
+      const float wp = mode == 0 ? q.sa / (q.sx * q.sx) : mode == 1 ? q.c * q.sb / (q.sa * q.sa) : end / q.sb;
+      const float wo = mode == 1 ? q.b * q.sb / q.sa : q.a * end;
 #pragma unroll 1
       for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
         const int ti = t / tn, tj = t % tn;
         const int N = min(128, (mode == 2 ? sh.n16 : sh.m16) - 128 * tj);
-        float acc[2][32];
+        const bool here = c < N;
+        const size_t band = (size_t)ti * blocks * kBlk;
+        float acc[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) acc[k] = 0.f;
+        const int mine = mode == 1 ? 2 * tj + (c >> 6) : 2 * ti + (row >> 6);   // the chunk with this warp's part
 #pragma unroll 1
-        for (int s0 = 0; s0 < chunks; s0 += kSegment, ++seg) {
-          if (!(ok = wait_bar(&bar.acc_full[seg & 1], (seg >> 1) & 1, gave_up))) break;
+        for (int kc = 0; kc < chunks; ++kc) {
+          if (old_chunk(mode, ti, tj, kc)) {
+            if (here && kc == mine) {
+              if (!(ok = wait_bar(&bar.full[st], parity >> st & 1u, gave_up))) break;
+              const char* from = ring + st * stage_bytes;
+              size_t lo = full_rows;
+              if (mode == 2) {
+                from += 2 * full_rows + (c >> 6) * (kBlk / 2);
+                lo = kBlk;
+              }
+              float x[32];
+              load_pairs32(from, from + lo, 128, mode == 1 ? row : row & 63, c & 63, x);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int c = half * 64 + i * 32;
-            if (c >= N) continue;
-            float v[32];
-            tmem_ld32(tmem + (seg & 1) * 256 + 128 + lanes + c, v);
-            if (s0 == 0) {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) acc[i][k] = v[k];
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; ++k) acc[i][k] += v[k];
+              for (int k = 0; k < 32; ++k) acc[k] = fmaf(wo, x[k], acc[k]);
             }
-            tmem_ld32(tmem + (seg & 1) * 256 + lanes + c, v);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.old_read[st]);
+          }
+          parity ^= 1u << st;
+          if (++st == stages) st = 0;
+          if ((kc + 1) % kSegment && kc + 1 < chunks) continue;
+          if (!(ok = wait_bar(&bar.acc_full[seg & 1], (seg >> 1) & 1, gave_up))) break;
+          if (here) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) acc[i][k] += v[k];
+            for (int h = 0; h < 4; ++h) {   // small terms and hi hi, 16 columns each
+              float v[16];
+              tmem_ld16(tmem + (seg & 1) * 256 + (h & 1 ? 0 : 128) + lanes + c + (h >> 1) * 16, v);
+              const float l = h & 1 ? loss : 0.f;
+#pragma unroll
+              for (int k = 0; k < 16; ++k) acc[(h >> 1) * 16 + k] = fmaf(wp, fmaf(v[k], l, v[k]), acc[(h >> 1) * 16 + k]);
+            }
           }
           fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bar.acc_empty[seg & 1]);
+          ++seg;
         }
         if (!ok) break;
-        const size_t band = (size_t)ti * blocks * kBlk;
+        // The block's last tile of the product leaves through the ring, which is
+        // idle until the group has met, hi and lo at once; others, while the ring
+        // serves the next tile, through the two blocks behind it, one after the other.
+        const uint32_t bytes = sh.band_rows(ti) * 128;
+        const bool ring_free = t + group >= sh.tiles(mode);
+        uint32_t words[2][16];   // hi and lo of 32 columns; at the end float32 columns 0 .. 15 and 16 .. 31
+        auto write = [&](char* at, int part) {
+          if (!here) return;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = half * 64 + i * 32;
-          if (c >= N) continue;
-          const int c0 = 128 * tj + c;
-          if (mode == 0) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) acc[i][k] *= fA;
-          } else {
-            float o[32];   // this thread's own writes, or the first image
-            load_pairs32(old + band, old + size + band, 128, row, c0, o);
-            const float fo = mode == 1 ? fbA : q.a, fd = mode == 1 ? fcAA : fX;
-#pragma unroll
-            for (int k = 0; k < 32; ++k) acc[i][k] = fmaf(fo, o[k], fd * acc[i][k]);
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t o = last ? raw_offset(row, c + 4 * j, kBlk) : sw128_offset(row, c + 8 * j, 128);
+            *reinterpret_cast<uint4*>(at + o) = make_uint4(words[part][4 * j], words[part][4 * j + 1],
+                                                           words[part][4 * j + 2], words[part][4 * j + 3]);
           }
-          if (p + 1 == phases) {
+        };
+        auto hand_on = [&]() {   // true in warp 2 when all have written
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.written);
+          if (warp == 2) ok = wait_bar(&bar.written, outs, gave_up);
+          ++outs;
+          return warp == 2 && ok;
+        };
+        auto send = [&](char* from, int part) {
+          char* const to = dst + part * size + band + (size_t)2 * tj * kBlk;
+          bulk_copy_s2g(to, from, bytes);
+          if (N > 64) bulk_copy_s2g(to + kBlk, from + kBlk, bytes);
+        };
+        auto emit = [&]() {
+          if (last) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) acc[i][k] *= back;
-            store_raw16(dst + band, dst + size + band, 128, row, c0, acc[i]);
-            store_raw16(dst + band, dst + size + band, 128, row, c0 + 16, acc[i] + 16);
+            for (int k = 0; k < 32; ++k) words[k >> 4][k & 15] = __float_as_uint(acc[k]);
           } else {
-            store_pairs16(dst + band, dst + size + band, 128, row, c0, acc[i]);
-            store_pairs16(dst + band, dst + size + band, 128, row, c0 + 16, acc[i] + 16);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) split2(acc[2 * k], acc[2 * k + 1], words[0][k], words[1][k]);
           }
-        }
+          if (ring_free) {
+            write(ring, 0);
+            write(ring + 2 * kBlk, 1);
+            if (hand_on() && lane == 0) {
+              send(ring, 0);
+              send(ring + 2 * kBlk, 1);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+            __syncwarp();
+            return;
+          }
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            if (frees && !(ok = wait_bar(&bar.out_free, frees - 1, gave_up))) return;
+            ++frees;
+            write(out, part);
+            if (hand_on() && lane == 0) {
+              send(out, part);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              mbar_arrive(&bar.out_free);
+            }
+            __syncwarp();
+          }
+        };
+        emit();
+        if (!ok) break;
       }
       if (!ok) break;
-      __threadfence();
-      fence_proxy_async_all();
+      if (warp == 2 && lane == 0) {
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        fence_proxy_async_all();
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(w.counter + p) : "memory");
+      }
       __syncwarp();
-      if (lane == 0) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(w.counter + p) : "memory");
     }
+    if (!ok && warp == 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   fence_before_sync();
