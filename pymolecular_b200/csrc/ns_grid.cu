@@ -13,9 +13,9 @@
 // A block computes 128 x 128 tiles of its group's products: one warp streams
 // operands through a ring of 64-column stages, one issues the products, sixteen
 // turn accumulators (two, used in turn) into blocks of an image, which leave
-// through shared memory as bulk copies: 16-byte stores to global memory and the
-// fence behind them took 8,300 cycles a tile, these copies REPLACE_ME.  Blocks of a
-// group meet after each product at a counter in global memory; only the copies
+// through shared memory as bulk copies (16-byte stores from the accumulators'
+// rows and the fence behind them took 8,300 cycles a tile, these 6,300).  Blocks
+// of a group meet after each product at a counter in global memory; only the copies
 // of the next product wait for it.  The wait is bounded, and the launch is
 // cooperative, so all blocks are resident.
 //
@@ -25,7 +25,7 @@
 // Sums in tensor memory are rounded towards zero at every instruction, by the
 // size of the sum so far.  So lo hi + hi lo has an accumulator of its own, and
 // an accumulator takes at most 128 terms, in 8 instructions; the pieces are
-// added in float32 registers.
+// added in float32 registers, and what truncation loses on average is added back.
 #include <atomic>
 
 #include "ns_tiles.cuh"
@@ -44,7 +44,6 @@ constexpr int kThreads = 64 + 32 * kReaders;   // and one of copies, one of prod
 constexpr int kMaxStages = 8;
 constexpr int kBlk = 16384;            // bytes of a 128 x 64 block
 constexpr int kRing = 12 * kBlk;
-constexpr int kSegment = 2;            // 64-column chunks of one accumulator
 constexpr size_t kSmem = kRing + 2 * kBlk + 1024;   // the ring, the blocks on their way out, alignment
 
 __host__ __device__ inline int up(int a, int b) { return (a + b - 1) / b; }
@@ -91,6 +90,9 @@ struct Shape {
     const int s = kRing / stage_bytes(mode);
     return s < kMaxStages ? s : kMaxStages;
   }
+  // 64-column chunks of one accumulator.  One band has few accumulators to add up,
+  // and shorter ones (128 x 2000: error 2.6e-6 with two chunks, 1.8e-6 with one) cost it little.
+  __host__ __device__ int segment() const { return bands > 1 ? 2 : 1; }
   __host__ __device__ int k16(int mode) const { return (mode == 0 ? n16 : m16) >> 4; }
 };
 
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = tmem_s;
-  const int phases = 3 * q.steps;
+  const int phases = 3 * q.steps, segment = sh.segment();
   bool ok = true;
 
   if (warp == 0) {
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
         const uint32_t idesc = make_idesc_f16(128, min(128, (mode == 2 ? sh.n16 : sh.m16) - 128 * tj), 0, mode == 2);
 #pragma unroll 1
         for (int kc = 0; kc < chunks && ok; ++kc) {
-          const bool start = kc % kSegment == 0;
+          const bool start = kc % segment == 0;
           // the accumulator's last user has been read
           if (start && !(ok = wait_bar(&bar.acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, gave_up))) break;
           if (!(ok = wait_bar(&bar.full[st], parity >> st & 1u, gave_up))) break;
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
                                 idesc, !(start && pr != 1 && j == 0));
           if (one) mma_commit(&bar.empty[st]);
           if (++st == stages) st = 0;
-          if ((kc + 1) % kSegment == 0 || kc + 1 == chunks) {
+          if ((kc + 1) % segment == 0 || kc + 1 == chunks) {
             if (one) mma_commit(&bar.acc_full[seg & 1]);
             ++seg;
           }
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     // one 32-column piece
     const int row = (warp & 3) * 32 + lane, c = ((warp - 2) >> 2) * 32;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const float loss = ns_mean_loss(4 * kSegment);
+    const float loss = ns_mean_loss(4 * segment);
     int seg = 0, outs = 0, frees = 0;
     uint32_t parity = 0;   // of each stage's next filling
 #pragma unroll 1
@@ -452,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           }
           parity ^= 1u << st;
           if (++st == stages) st = 0;
-          if ((kc + 1) % kSegment && kc + 1 < chunks) continue;
+          if ((kc + 1) % segment && kc + 1 < chunks) continue;
           if (!(ok = wait_bar(&bar.acc_full[seg & 1], (seg >> 1) & 1, gave_up))) break;
           if (here) {
 #pragma unroll
@@ -485,6 +487,11 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
                                                            words[part][4 * j + 2], words[part][4 * j + 3]);
           }
         };
+        auto meet = [&]() {   // of the readers
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.written);
+          return wait_bar(&bar.written, outs++, gave_up);
+        };
         auto hand_on = [&]() {   // true in warp 2 when all have written
           fence_proxy_async();
           __syncwarp();
@@ -507,6 +514,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
             for (int k = 0; k < 16; ++k) split2(acc[2 * k], acc[2 * k + 1], words[0][k], words[1][k]);
           }
           if (ring_free) {
+            // every reader has taken its part of the old tile out of the ring
+            if (mode != 0 && !(ok = meet())) return;
             write(ring, 0);
             write(ring + 2 * kBlk, 1);
             if (hand_on() && lane == 0) {
