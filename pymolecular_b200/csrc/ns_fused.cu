@@ -118,8 +118,7 @@ __device__ __forceinline__ double take_in(const NsItem& it, const NsScalars& q, 
           }
           unit_store(mom, ld_mom, u, rows, cols, m[i]);
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ss = fma((double)g[i][k], (double)g[i][k], ss);
+        ss += squares(g[i]);
         // rows past the matrix get the zeros that are there already
         if (u.c < cols) unit_to_raw(Xh, Xl, blk, turn, u, g[i]);
 #pragma unroll

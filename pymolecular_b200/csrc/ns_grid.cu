@@ -129,8 +129,7 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Gr
       }
       unit_store(it.mom, it.ld_mom, u, it.rows, it.cols, mo);
     }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) ss = fma((double)v[k], (double)v[k], ss);
+    ss += squares(v);
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);

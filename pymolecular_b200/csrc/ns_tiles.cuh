@@ -155,12 +155,52 @@ __device__ __forceinline__ void unit_store(T* p, int64_t ld, const Unit& u, int 
     if (k < n) *p = ns_from<T>(v[k]);
 }
 
-// The scale 1 / (norm + eps) as pre * f: a power of two first, so that f is a
-// float32 at any norm.
+// The sum of 8 squares, for a sum in float64: in float32 where that neither
+// overflows nor loses small ones (conversions and float64 products would cost
+// more than the rest of an element).
+__device__ __forceinline__ double squares(const float (&v)[8]) {
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) s = fmaf(v[k], v[k], s);
+  if (s > 0x1p-80f && s < 0x1p100f) return (double)s;
+  uint32_t any = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) any |= __float_as_uint(v[k]) << 1;
+  if (!any) return 0.0;
+  double d = 0.0;
+#pragma unroll 1
+  for (int k = 0; k < 8; ++k) {
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x = j == k ? v[j] : x;
+    d = fma((double)x, (double)x, d);
+  }
+  return d;
+}
+
+// x 2^-e for |e| < 1000.
+__device__ __forceinline__ float scaled_down(double x, int e) {
+  return (float)(x * __hiloint2double((1023 - e) << 20, 0));
+}
+// 1 / (sqrt(ss) + eps) as pre * f, so that both are float32 at any norm: norm and
+// eps are brought near 1 by the power of two h of the larger, and half of it goes
+// to each factor.  Float32 arithmetic: a float64 square root and division took
+// 3,000 cycles of a block's time.
 __device__ __forceinline__ void norm_scale(double ss, double eps, float& pre, float& f) {
-  const double inv = 1.0 / (sqrt(ss) + eps);
-  pre = inv > 1.0 ? 0x1p64f : inv < 0x1p-64 ? 0x1p-64f : 1.f;
-  f = (float)(inv / (double)pre);
+  const int e = ((__double2hiint(ss) >> 20) & 0x7ff) - 1023;   // -1023: zero; 1024: infinity or NaN
+  if (e == 1024) {
+    pre = 1.f;
+    f = (float)(1.0 / ss);
+    return;
+  }
+  const int eh = ((__double2hiint(eps) >> 20) & 0x7ff) - 1023;
+  int h = max(e >> 1, eh);
+  h = min(max(h, -200), 200);
+  const float norm = e == -1023 ? 0.f : ldexpf(sqrtf(scaled_down(ss, e & ~1)), max((e >> 1) - h, -200));
+  const float t = 1.f / (norm + scaled_down(eps, h));
+  const int h1 = h / 2;
+  pre = ldexpf(1.f, -h1);
+  f = ldexpf(t, h1 - h);
 }
 
 // ---- waits -------------------------------------------------------------------

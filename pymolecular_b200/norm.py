@@ -21,7 +21,7 @@ def _forward(x, weight, bias, eps, stats):
     """y and, where asked for, the (rows, 2) mean and 1 / sqrt(var + eps)."""
     rows, cols = x.shape
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    kept = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if stats else None
+    kept = x.new_empty((rows, 2), dtype=torch.float32) if stats else None
     p = weight if weight is not None else bias
     with nat.device_of(x):
         nat.check(nat.lib().egnn_layer_norm_fwd(rows, cols, x.data_ptr(), x.stride(0), DTYPES[x.dtype], nat.ptr(weight),
@@ -44,10 +44,10 @@ def _backward(ctx, dy):
         if need_w:
             dw = torch.empty_like(weight)
         if need_b:
-            db = torch.empty(cols, dtype=pdt, device=x.device)
+            db = x.new_empty(cols, dtype=pdt)
         if need_w or need_b:
             nbytes = lib.egnn_layer_norm_workspace_size(rows, cols)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
         nat.check(lib.egnn_layer_norm_bwd(rows, cols, x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0),
                                           DTYPES[x.dtype], nat.ptr(weight), DTYPES[pdt], stats.data_ptr(), nat.ptr(dx),
                                           nat.ptr(dw), nat.ptr(db), nat.ptr(ws), nbytes, nat.stream_ptr()),

@@ -151,7 +151,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
         pp, pm = p.data_ptr(), m.data_ptr()
         if rows * cols:
             written += (pp, pm)
-        fields += (pp, g.data_ptr(), pm, ldp, ldg, ldm, rows, cols, max(1.0, rows / max(cols, 1)) ** 0.5, 0)
+        fields += (pp, g.data_ptr(), pm, ldp, ldg, ldm, rows, cols,
+                   (rows / cols) ** 0.5 if rows > cols > 0 else 1.0, 0)
     if len(set(written)) < len(written):   # other tensors on the same memory
         raise ValueError("a parameter or momentum buffer is given twice")
     options = nat.MuonOptions(_options(steps, *coefficients, eps), momentum, weight_decay,
