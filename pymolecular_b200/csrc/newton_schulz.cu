@@ -10,6 +10,7 @@
 // block; a larger one by a group of blocks, through L2.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "newton_schulz.cuh"
 
@@ -65,6 +66,10 @@ int scalars(const char* what, const egnn_ns_options& o, NsScalars& q) {
   q.c = (float)o.c;
   q.eps = o.eps;
   q.steps = o.steps;
+  // the debugging aid of the edge kernels' waits (read at every call): 0 makes the readers give up at once
+  const char* polls = std::getenv("EGNN_DEBUG_WAIT_POLLS");
+  const long limit = polls && *polls ? std::strtol(polls, nullptr, 10) : -1;
+  q.wait_polls = limit < 0 ? 1 << 22 : (int)std::min<long>(limit, 1L << 22);
   q.sx = scale_for(most);
   q.sa = scale_for(most * most);
   q.sb = scale_for(std::fabs(o.b) * most * most + std::fabs(o.c) * most * most * most * most);

@@ -40,6 +40,7 @@ struct NsScalars {
   const float* lr_device;
   int nesterov;
   int steps;
+  int wait_polls;           // limit of the accumulator readers' waits
 };
 
 __device__ __forceinline__ float ns_float(float v) { return v; }

@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
 #pragma unroll 1
     for (int step = 0; step < q.steps && ok; ++step) {
       float v[32], w[32];
-      if (!(ok = wait_bar(&bar.a_done, step, gave_up))) break;
+      if (!(ok = wait_bar(&bar.a_done, step, gave_up, q.wait_polls))) break;
       if (a_here) {
         tmem_ld32(tA + lanes + piece * 32, v);
         for (int j = 1; j < sums; ++j) {

@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           parity ^= 1u << st;
           if (++st == stages) st = 0;
           if ((kc + 1) % segment && kc + 1 < chunks) continue;
-          if (!(ok = wait_bar(&bar.acc_full[seg & 1], (seg >> 1) & 1, gave_up))) break;
+          if (!(ok = wait_bar(&bar.acc_full[seg & 1], (seg >> 1) & 1, gave_up, q.wait_polls))) break;
           if (here) {
 #pragma unroll
             for (int h = 0; h < 4; ++h) {   // small terms and hi hi, 16 columns each

@@ -204,13 +204,14 @@ __device__ __forceinline__ void norm_scale(double ss, double eps, float& pre, fl
 }
 
 // ---- waits -------------------------------------------------------------------
+constexpr int kWaitPolls = 1 << 22;
 // Bounded wait, the same answer in the whole warp; false when it or another
 // warp's wait ran out.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* gave_up, int polls = kWaitPolls) {
   bool ok = false;
-  for (uint32_t i = 0; i < (1u << 22) && !ok; ++i) {
+  for (int i = 0; i < polls && !ok; ++i) {
     ok = tc::mbar_try_wait(bar, parity & 1u);
-    if (!ok && (i & 255u) == 255u && *gave_up) break;
+    if (!ok && (i & 255) == 255 && *gave_up) break;
   }
   ok = __all_sync(0xffffffffu, ok);
   if (!ok) *gave_up = 1;

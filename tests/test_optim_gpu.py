@@ -14,7 +14,8 @@ import math
 import pytest
 import torch
 
-from pymolecular_b200 import CSR, EGNN, Muon, graph_sum_mse, muon_step, orthogonalize
+from pymolecular_b200 import CSR, EGNN, Muon, graph_sum_mse, layer_norm, muon_step, orthogonalize
+from pymolecular_b200 import _native as nat
 from pymolecular_b200.datasets import molecules
 from pymolecular_b200.graphs import GraphedStep
 from pymolecular_b200.optim import COEFFICIENTS
@@ -314,3 +315,62 @@ def test_two_streams_at_once(cuda_device):
     for k in range(2):
         for outs in got[k]:
             assert all(torch.equal(a, b) for a, b in zip(outs, want[k]))
+
+
+def test_waits_that_run_out_are_reported_and_the_context_stays_usable(cuda_device, monkeypatch):
+    """EGNN_DEBUG_WAIT_POLLS=0 makes the accumulator readers of both kernels
+    give up on their first wait (nothing hangs: the products complete and are
+    drained); the status says so once, and later calls give the same results."""
+    lib = nat.lib()
+    g = torch.Generator(device="cuda").manual_seed(12)
+    mats = [_gradient(r, c, g) for r, c in [(64, 129), (128, 257), (200, 333), (256, 513)]]
+    monkeypatch.delenv("EGNN_DEBUG_WAIT_POLLS", raising=False)
+    want = orthogonalize(mats)
+    assert lib.egnn_device_status(nat.stream_ptr()) == nat.EGNN_OK, nat.last_error()
+    for only in (mats[:2], mats[2:]):   # one kernel, then the other
+        monkeypatch.setenv("EGNN_DEBUG_WAIT_POLLS", "0")
+        orthogonalize(only)
+        assert lib.egnn_device_status(nat.stream_ptr()) == nat.EGNN_ERR_CUDA and "timed out" in nat.last_error()
+        assert lib.egnn_device_status(nat.stream_ptr()) == nat.EGNN_OK
+        monkeypatch.delenv("EGNN_DEBUG_WAIT_POLLS")
+        assert all(torch.equal(a, b) for a, b in zip(orthogonalize(mats), want))
+
+
+def test_many_matrices_and_two_graphs_that_share_a_pool(cuda_device):
+    """More matrices than one launch takes, of both kernels, and two captured
+    calls whose workspaces come from one pool, replayed in turn."""
+    g = torch.Generator(device="cuda").manual_seed(13)
+    mats = [_gradient(*s, g) for s in [(40, 60), (130, 150)] * 70]
+    want = orthogonalize(mats)
+    assert all(torch.equal(o, orthogonalize(t)) for t, o in list(zip(mats, want))[::23])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        orthogonalize(mats[:4])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for k in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[k], pool=graphs[0].pool() if k else None):
+            outs.append(orthogonalize(mats[2 * k:2 * k + 2]))
+    for _ in range(3):
+        for k in (0, 1):
+            graphs[k].replay()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(outs[k], want[2 * k:2 * k + 2]))
+
+
+def test_rows_far_apart_and_an_offset_past_32_bits(cuda_device):
+    """Row strides that put a matrix over more than 4 GB."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    store = torch.empty(34 * (1 << 27), dtype=torch.bfloat16, device="cuda")   # 9.1 GB
+    far = store.as_strided((33, 50), (1 << 27, 1))
+    far.copy_(_gradient(33, 50, g))
+    near = far.clone()
+    assert torch.equal(orthogonalize(far), orthogonalize(near))
+    x = store.as_strided((33, 64), (1 << 27, 1))
+    x.normal_(generator=g)
+    layer = torch.nn.LayerNorm(64, device="cuda")
+    with torch.no_grad():
+        assert torch.equal(layer_norm(x, layer), layer_norm(x.clone(), layer))
