@@ -368,7 +368,7 @@ class Problem:
 KERNELS = ("edge_bwd", "edge_fwd", "node_pass", "src_pass", "edge_fixup", "part_reduce", "node_gemm", "node_wgrad",
            "gemm_small",
            "linear_small", "wgrad_small", "colsum", "gemm_reduce", "prep", "edge_rows_gemm", "edge_rows_wgrad",
-           "edge_rows_u", "edge_rows_agg", "edge_rows_wimg", "graph_mse")
+           "edge_rows_u", "edge_rows_agg", "edge_rows_wimg", "graph_mse", "layer_norm", "newton_schulz")
 
 
 def measure(prob, args, world, dev, steps, warmup, graphs=True, e2e=True):

@@ -37,14 +37,10 @@ def _backward(ctx, dy):
     need_x, need_w, need_b, _ = ctx.needs_input_grad
     pdt = weight.dtype if weight is not None else ctx.bias_dtype or torch.float32
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
-    dw = db = ws = None
-    nbytes = 0
-    lib = nat.lib()
+    dw = torch.empty_like(weight) if need_w else None
+    db = x.new_empty(cols, dtype=pdt) if need_b else None
+    lib, ws, nbytes = nat.lib(), None, 0
     with nat.device_of(x):
-        if need_w:
-            dw = torch.empty_like(weight)
-        if need_b:
-            db = x.new_empty(cols, dtype=pdt)
         if need_w or need_b:
             nbytes = lib.egnn_layer_norm_workspace_size(rows, cols)
             ws = x.new_empty(nbytes, dtype=torch.uint8)

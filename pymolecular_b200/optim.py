@@ -69,32 +69,42 @@ def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = S
     device = mats[0].get_device()
     if device < 0:
         raise ValueError("orthogonalize takes CUDA tensors (pymolecular_b200 has no CPU path)")
-    groups, sizes, copies = {}, [], []
+    groups, sizes, ptrs, strides, copies = {}, [], [], [], []
     for k, t in enumerate(mats):
-        if t.dim() != 2:
+        size, code = t.shape, DTYPES.get(t.dtype)
+        if len(size) != 2:
             raise ValueError("orthogonalize takes matrices")
         if t.get_device() != device:
             raise ValueError("the matrices of a call must be on one device")
-        size, dtype = t.shape, t.dtype
-        if dtype not in DTYPES:
-            raise TypeError(f"matrices must be float32, bfloat16 or float16, got {dtype}")
-        if not t.is_contiguous() and not (t.stride(1) == 1 and t.stride(0) >= size[1]):
-            t = t.contiguous()
-            copies.append(t)   # lives until the launch
+        if code is None:
+            raise TypeError(f"matrices must be float32, bfloat16 or float16, got {t.dtype}")
+        stride = size[1]
+        if not t.is_contiguous():
+            if t.stride(1) == 1 and t.stride(0) >= stride:
+                stride = t.stride(0)
+            else:
+                t = t.contiguous()
+                copies.append(t)   # lives until the launch
         sizes += size
-        groups.setdefault((size, dtype), []).append((k, t))
-    fields, out = [None] * len(mats), [None] * len(mats)
-    for (size, dtype), members in groups.items():
-        made = torch.empty((len(members), *size), dtype=dtype, device=device)
+        ptrs.append(t.data_ptr())
+        strides.append(stride)
+        key = (size, code)
+        if key in groups:
+            groups[key].append(k)
+        else:
+            groups[key] = [k]
+    fields, out = [0] * (6 * len(mats)), [None] * len(mats)
+    for (size, code), members in groups.items():
         rows, cols = size
-        at, step, code = made.data_ptr(), rows * cols * made.element_size(), DTYPES[dtype]
-        for (k, t), o in zip(members, made.unbind(0)):
+        made = torch.empty((len(members), rows, cols), dtype=mats[members[0]].dtype, device=device)
+        at, step, both = made.data_ptr(), rows * cols * made.element_size(), rows | cols << 32
+        for k, o in zip(members, made.unbind(0)):
             out[k] = o
-            fields[k] = (t.data_ptr(), at, t.stride(0), cols, rows | cols << 32, code)
+            fields[6 * k:6 * k + 6] = ptrs[k], at, strides[k], cols, both, code
             at += step
     with nat.device_of(mats[0]):
         ws, nbytes = _workspace(sizes, device)
-        items = struct.pack("%dQ" % (6 * len(mats)), *[v for f in fields for v in f])
+        items = struct.pack("%dQ" % len(fields), *fields)
         nat.check(nat.lib().egnn_orthogonalize(len(mats), items, C.byref(_options(steps, *coefficients, eps)),
                                                ws.data_ptr(), nbytes, nat.stream_ptr()), "egnn_orthogonalize")
     if not isinstance(g, torch.Tensor):
