@@ -376,7 +376,8 @@ EGNN_API int egnn_orthogonalize(int64_t count, const egnn_matrix* m, const egnn_
                                 size_t workspace_bytes, void* stream);
 
 /* One weight matrix of egnn_muon_step (float32, row-major, row strides in
- * elements); no two of a call's weights and momenta may overlap. */
+ * elements); no two of a call's weights and momenta may overlap, nor one of
+ * them a gradient. */
 typedef struct {
   float* weight;
   const float* grad;

@@ -118,7 +118,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
               coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = EPS) -> None:
     """One momentum step with orthogonalised updates, in place on `params` and
     their momenta `buffers` (float32 CUDA matrices with dense rows, no two of
-    them overlapping).  `lr` is a number or a one-element float32 CUDA tensor,
+    them overlapping each other or a gradient).  `lr` is a number or a one-element float32 CUDA tensor,
     which a captured step reads at each replay."""
     params, grads, buffers = list(params), list(grads), list(buffers)
     if not len(params) == len(grads) == len(buffers):
@@ -134,7 +134,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
     if on_device and (lr.numel() != 1 or lr.dtype != torch.float32 or lr.get_device() != device):
         raise ValueError("lr must be a number or one float32 on the parameters' device")
     f32 = torch.float32
-    sizes, fields, written, copies = [], [], [], []
+    sizes, fields, written, read, copies = [], [], [], [], []
     for k, (p, g, m) in enumerate(zip(params, grads, buffers)):
         size = p.shape
         if len(size) != 2 or g.shape != size or m.shape != size:
@@ -158,13 +158,17 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
                 g = g.contiguous()
                 copies.append(g)   # lives until the launch
         sizes += size
-        pp, pm = p.data_ptr(), m.data_ptr()
+        pp, pg, pm = p.data_ptr(), g.data_ptr(), m.data_ptr()
         if rows * cols:
             written += (pp, pm)
-        fields += (pp, g.data_ptr(), pm, ldp, ldg, ldm, rows, cols,
+            read.append(pg)
+        fields += (pp, pg, pm, ldp, ldg, ldm, rows, cols,
                    (rows / cols) ** 0.5 if rows > cols > 0 else 1.0, 0)
-    if len(set(written)) < len(written):   # other tensors on the same memory
+    places = set(written)
+    if len(places) < len(written):   # other tensors on the same memory
         raise ValueError("a parameter or momentum buffer is given twice")
+    if not places.isdisjoint(read):
+        raise ValueError("a gradient lies where a parameter or momentum buffer is written")
     options = nat.MuonOptions(_options(steps, *coefficients, eps), momentum, weight_decay,
                               0.0 if on_device else lr, nat.ptr(lr) if on_device else None, int(nesterov), 0)
     with nat.device_of(params[0]):
@@ -194,11 +198,14 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"weight_decay must not be negative, got {weight_decay}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       steps=steps, coefficients=tuple(coefficients), eps=eps))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() != 2 or p.dtype != torch.float32:
-                    raise ValueError(f"Muon takes float32 matrices, got {tuple(p.shape)} {p.dtype} (Muon.split gives "
-                                     "them and the rest apart)")
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2 or p.dtype != torch.float32:
+                del self.param_groups[-1]
+                raise ValueError(f"Muon takes float32 matrices, got {tuple(p.shape)} {p.dtype} (Muon.split gives them and "
+                                 "the rest apart)")
 
     @staticmethod
     def split(params: Iterable[torch.Tensor]) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:

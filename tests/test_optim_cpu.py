@@ -142,6 +142,12 @@ def test_muon_arguments_and_split():
         Muon(rest)
     with pytest.raises(ValueError, match="matrices"):
         Muon([nn.Parameter(torch.zeros(4, 4, dtype=torch.float64))])
+    opt = Muon(mats[:2])
+    with pytest.raises(ValueError, match="matrices"):
+        opt.add_param_group({"params": rest[:1]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": mats[2:], "lr": 0.1})
+    assert len(opt.param_groups) == 2
 
 
 def test_node_norm_keeps_the_other_parameters():

@@ -374,3 +374,30 @@ def test_rows_far_apart_and_an_offset_past_32_bits(cuda_device):
     layer = torch.nn.LayerNorm(64, device="cuda")
     with torch.no_grad():
         assert torch.equal(layer_norm(x, layer), layer_norm(x.clone(), layer))
+
+
+def test_tensors_that_a_step_would_spoil_are_refused(cuda_device):
+    def t(*shape, dtype=torch.float32):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+    store = t(40, 40)
+    w, g, m = t(40, 40), t(40, 40), t(40, 40)
+    for args in (([w, w], [g, g], [m, t(40, 40)]), ([w], [g], [w]), ([store], [g], [store.view(40, 40)]),
+                 ([w], [m.view(40, 40)], [m]), ([w], [w], [m]), ([t(40, 41)[:, 1:].t()], [g], [m]), ([w], [g], [m.t()[:, ::2]]),
+                 ([w], [g], [m.cpu()]), ([w], [g], [m], torch.tensor(0.1)), ([w], [g], [m], t(2)),
+                 ([t(40)], [t(40)], [t(40)]), ([t(1100, 1100)], [t(1100, 1100)], [t(1100, 1100)])):
+        with pytest.raises(ValueError):
+            muon_step(*args[:3], lr=args[3] if len(args) > 3 else 0.1)
+    for args in (([t(4, 4, dtype=torch.float64)], [t(4, 4)], [t(4, 4)]), ([w], [g.bfloat16()], [m])):
+        with pytest.raises(TypeError):
+            muon_step(*args, lr=0.1)
+    with pytest.raises(ValueError, match="one device"):
+        orthogonalize([w, w.cpu()])
+    with pytest.raises(TypeError):
+        orthogonalize(t(4, 4, dtype=torch.float64))
+    with pytest.raises(ValueError, match="at most"):
+        orthogonalize(t(1030, 1030))
+    with pytest.raises(nat.EgnnError, match="grow"):
+        orthogonalize(w, coefficients=(5.0, 0.0, 0.0))
+    muon_step([], [], [], lr=0.1)
+    assert not any(x.any() for x in (w, g, m, store))
