@@ -326,11 +326,14 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
     const int row = (warp & 3) * 32 + lane, piece = warp >> 2;
     const bool rows_here = (warp & 3) * 32 < R;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    // this thread's pieces of X (128 columns apart) and of A
+    const uint32_t xh = row_at(smem_u32(Xh), R, row, piece * 32), ah = row_at(smem_u32(Ah), R, row, piece * 32);
     for (int k = 0; k < chunks; ++k) {
       const int c0 = k * kSlotCols + piece * 32;
+      const uint32_t hi = xh + k * (2 * R * 128), lo = hi + xt;
       float v[32];
       if (rows_here && c0 < n16) {
-        load_raw32(Xh, Xl, R, row, c0, v);
+        load_raw32(hi, lo, v);
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = v[j] * pre * f;
       }
@@ -338,11 +341,11 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
       for (int h = 0; h < 2; ++h) {
         if (rows_here && c0 < n16) {
           if (q.steps == 0) {
-            store_raw16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+            store_raw16(hi, lo, h, v + 16 * h);
           } else {
 #pragma unroll
             for (int j = 16 * h; j < 16 * h + 16; ++j) v[j] *= q.sx;
-            store_pairs16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+            store_pairs16(hi, lo, h, v + 16 * h);
           }
         }
         arrive(&bar.x_ready[k][h]);
@@ -374,12 +377,12 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (a_here) store_pairs16(Ah, Al, R, row, piece * 32 + 16 * h, v + 16 * h);
+        if (a_here) store_pairs16(ah, ah + at, h, v + 16 * h);
         arrive(&bar.a_ready[h]);
       }
       if (!(ok = wait_bar(&bar.aa_done, step, gave_up))) break;
       if (a_here) {
-        load_pairs32(Ah, Al, R, row, piece * 32, w);   // this thread's own
+        load_pairs32(ah, ah + at, w);   // this thread's own
         tmem_ld32(tAA + lanes + piece * 32, v);
 #pragma unroll
         for (int k = 0; k < 32; ++k) w[k] = fmaf(fbA, w[k], fcAA * fmaf(v[k], loss_m, v[k]));
@@ -404,9 +407,10 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
         if (!(ok = wait_bar(&bar.slot_done[slot], slot_use(step, k), gave_up))) break;
         const int c0 = k * kSlotCols + piece * 32;
         const bool here = rows_here && c0 < n16;
+        const uint32_t hi = xh + k * (2 * R * 128), lo = hi + xt;
         if (here) {
           tmem_ld32(tmem + lanes + slot * kSlotCols + piece * 32, v);
-          load_pairs32(Xh, Xl, R, row, c0, w);
+          load_pairs32(hi, lo, w);
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = fmaf(q.a, w[j], fX * fmaf(v[j], loss_m, v[j]));
         }
@@ -414,11 +418,11 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
         for (int h = 0; h < 2; ++h) {
           if (here) {
             if (step + 1 < q.steps) {
-              store_pairs16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+              store_pairs16(hi, lo, h, v + 16 * h);
             } else {
 #pragma unroll
               for (int j = 16 * h; j < 16 * h + 16; ++j) v[j] *= back;
-              store_raw16(Xh, Xl, R, row, c0 + 16 * h, v + 16 * h);
+              store_raw16(hi, lo, h, v + 16 * h);
             }
           }
           arrive(&bar.x_ready[k][h]);

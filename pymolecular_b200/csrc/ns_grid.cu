@@ -437,14 +437,11 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           if (old_chunk(mode, ti, tj, kc)) {
             if (here && kc == mine) {
               if (!(ok = wait_bar(&bar.full[st], parity >> st & 1u, gave_up))) break;
-              const char* from = ring + st * stage_bytes;
-              size_t lo = full_rows;
-              if (mode == 2) {
-                from += 2 * full_rows + (c >> 6) * (kBlk / 2);
-                lo = kBlk;
-              }
+              const uint32_t stage = smem_u32(ring) + st * stage_bytes;
+              const uint32_t from = mode == 1 ? row_at(stage, 128, row, c & 63)
+                                              : row_at(stage + 2 * full_rows + (c >> 6) * (kBlk / 2), 128, row & 63, c & 63);
               float x[32];
-              load_pairs32(from, from + lo, 128, mode == 1 ? row : row & 63, c & 63, x);
+              load_pairs32(from, from + (mode == 1 ? full_rows : kBlk), x);
 #pragma unroll
               for (int k = 0; k < 32; ++k) acc[k] = fmaf(wo, x[k], acc[k]);
             }
@@ -479,12 +476,10 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
         uint32_t words[2][16];   // hi and lo of 32 columns; at the end float32 columns 0 .. 15 and 16 .. 31
         auto write = [&](char* at, int part) {
           if (!here) return;
+          const uint32_t to = row_at(smem_u32(at), 128, row, c);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t o = last ? raw_offset(row, c + 4 * j, kBlk) : sw128_offset(row, c + 8 * j, 128);
-            *reinterpret_cast<uint4*>(at + o) = make_uint4(words[part][4 * j], words[part][4 * j + 1],
-                                                           words[part][4 * j + 2], words[part][4 * j + 3]);
-          }
+          for (int j = 0; j < 4; ++j)
+            sts16(to ^ (j << 4), words[part][4 * j], words[part][4 * j + 1], words[part][4 * j + 2], words[part][4 * j + 3]);
         };
         auto meet = [&]() {   // of the readers
           __syncwarp();

@@ -10,66 +10,85 @@ namespace ns {
 
 using tc::sw128_offset;
 
+// hi + c and hi - c with hi one half of a word of two fp16, in float32.
+__device__ __forceinline__ float add_low(uint32_t w, float c) {
+  float d;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tadd.f32.f16 %0, a, %2;\n\t}" : "=f"(d) : "r"(w), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float add_high(uint32_t w, float c) {
+  float d;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tadd.f32.f16 %0, b, %2;\n\t}" : "=f"(d) : "r"(w), "f"(c));
+  return d;
+}
 // x, y as fp16 pairs hi + lo, x in the lower half of the words.
 __device__ __forceinline__ void split2(float x, float y, uint32_t& h, uint32_t& l) {
   const __half2 p = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(p);
-  const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
   h = *reinterpret_cast<const uint32_t*>(&p);
+  const __half2 r = __floats2half2_rn(-add_low(h, -x), -add_high(h, -y));
   l = *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// hi and lo tiles at (row, c0 .. c0 + 15) <- v.
-__device__ __forceinline__ void store_pairs16(char* hi, char* lo, int R, int row, int c0, const float* v) {
+// ---- 32 columns of a tile row in shared memory -----------------------------------
+// They are 4 chunks of 16 bytes in the hi tile and 4 in the lo tile, chunk j at the
+// row's address ^ (j << 4).  As float32 (before the first product and after the
+// last) the same bytes hold columns 0 .. 15 in hi and 16 .. 31 in lo.
+__device__ __forceinline__ uint32_t row_at(uint32_t tile, int R, int row, int c0) {
+  return tile + (c0 >> 6) * (R * 128) + (row << 7) + (((c0 >> 3 & 4) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// Columns 16 half .. + 15 as pairs.
+__device__ __forceinline__ void store_pairs16(uint32_t hi, uint32_t lo, int half, const float* v) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     uint32_t h[4], l[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) split2(v[8 * j + 2 * k], v[8 * j + 2 * k + 1], h[k], l[k]);
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    const uint32_t chunk = (2 * half + j) << 4;
+    sts16(hi ^ chunk, h[0], h[1], h[2], h[3]);
+    sts16(lo ^ chunk, l[0], l[1], l[2], l[3]);
   }
 }
-
-__device__ __forceinline__ void load_pairs32(const char* hi, const char* lo, int R, int row, int c0, float (&v)[32]) {
+__device__ __forceinline__ void load_pairs32(uint32_t hi, uint32_t lo, float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t at = sw128_offset(row, c0 + 8 * j, R);
-    const uint4 h = *reinterpret_cast<const uint4*>(hi + at), l = *reinterpret_cast<const uint4*>(lo + at);
+    const uint4 h = lds16(hi ^ (j << 4)), l = lds16(lo ^ (j << 4));
     const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&hh[k]));
-      const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&ll[k]));
-      v[8 * j + 2 * k] = p.x + r.x;
-      v[8 * j + 2 * k + 1] = p.y + r.y;
+      v[8 * j + 2 * k] = add_low(hh[k], add_low(ll[k], 0.f));
+      v[8 * j + 2 * k + 1] = add_high(hh[k], add_high(ll[k], 0.f));
     }
   }
 }
-
-// Before the first product and after the last, the bytes of 32 columns of a
-// row in both tiles hold them as float32: columns 0 .. 15 where the hi halves
-// are, 16 .. 31 where the lo halves are.  Offset of column c in its tile:
-__device__ __forceinline__ uint32_t raw_offset(int row, int c, uint32_t blk) {
-  return (c >> 6) * blk + (row << 7) + ((((c >> 3 & 4) | (c >> 2 & 3)) ^ (row & 7)) << 4) + ((c & 3) << 2);
-}
-__device__ __forceinline__ void store_raw16(char* hi, char* lo, int R, int row, int c0, const float* v) {
-  char* const t = c0 & 16 ? lo : hi;
+// Columns 16 half .. + 15 as float32.
+__device__ __forceinline__ void store_raw16(uint32_t hi, uint32_t lo, int half, const float* v) {
+  const uint32_t t = half ? lo : hi;
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    *reinterpret_cast<float4*>(t + raw_offset(row, c0 + 4 * j, R * 128)) =
-        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    sts16(t ^ (j << 4), __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+          __float_as_uint(v[4 * j + 3]));
 }
-__device__ __forceinline__ void load_raw32(const char* hi, const char* lo, int R, int row, int c0, float (&v)[32]) {
+__device__ __forceinline__ void load_raw32(uint32_t hi, uint32_t lo, float (&v)[32]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float4 x = *reinterpret_cast<const float4*>((j & 4 ? lo : hi) + raw_offset(row, c0 + 4 * j, R * 128));
-    v[4 * j] = x.x;
-    v[4 * j + 1] = x.y;
-    v[4 * j + 2] = x.z;
-    v[4 * j + 3] = x.w;
+    const uint4 x = lds16((j & 4 ? lo : hi) ^ ((j & 3) << 4));
+    v[4 * j] = __uint_as_float(x.x);
+    v[4 * j + 1] = __uint_as_float(x.y);
+    v[4 * j + 2] = __uint_as_float(x.z);
+    v[4 * j + 3] = __uint_as_float(x.w);
   }
+}
+// Offset of float32 column c in its tile.
+__device__ __forceinline__ uint32_t raw_offset(int row, int c, uint32_t blk) {
+  return (c >> 6) * blk + (row << 7) + ((((c >> 3 & 4) | (c >> 2 & 3)) ^ (row & 7)) << 4) + ((c & 3) << 2);
 }
 
 // A warp's share of a matrix in global memory: units of 8 rows x 32 columns,
