@@ -58,6 +58,13 @@ bool tensor_map_i32_1d(void* map, const int32_t* p, int64_t n, int box);
 // Bit of the current device (for per-device one-time setup flags).
 uint64_t device_bit();
 
+// ---- work beside the caller's stream -----------------------------------------
+// A stream of the library's own, beside `caller`, that waits for what has been
+// issued on `caller` so far; join_side makes `caller` wait for it.  Both are
+// event waits, which stream capture records.
+int fork_side(cudaStream_t caller, cudaStream_t* side);
+int join_side(cudaStream_t caller);
+
 // ---- programmatic dependent launch ------------------------------------------
 // Kernels on the layer's hot path are launched with launch_pdl: such a kernel
 // may start while its predecessor in the stream is still finishing.  It calls

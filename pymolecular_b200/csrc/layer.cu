@@ -486,6 +486,19 @@ void fill_common(EdgeCommon& a, const egnn_layer_desc* d, const egnn_graph* g, c
 }
 
 }  // namespace
+
+int fork_side(cudaStream_t caller, cudaStream_t* side) {
+  SideStream* ss = nullptr;
+  EGNN_TRY(side_stream(caller, &ss));
+  *side = ss->stream;
+  return stream_fork(caller, ss->stream, ss->ev[0]);
+}
+
+int join_side(cudaStream_t caller) {
+  SideStream* ss = nullptr;
+  EGNN_TRY(side_stream(caller, &ss));
+  return stream_fork(ss->stream, caller, ss->ev[6]);
+}
 }  // namespace egnn
 
 using namespace egnn;

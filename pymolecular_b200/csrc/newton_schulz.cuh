@@ -80,9 +80,9 @@ __host__ __device__ inline float ns_mean_loss(int instructions) {
 bool ns_fused_fits(int m, int n);
 // The matrices of the batch, one block each.
 int ns_fused(const NsBatch& b, const NsScalars& q, cudaStream_t s);
-// The matrices of the batch on the whole device, with workspace from `c`;
-// ns_grid_carve takes what one matrix needs.
-int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, cudaStream_t s);
+// The matrices of the batch on the whole device but `spare` SMs, with workspace
+// from `c`; ns_grid_carve takes what one matrix needs.
+int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, int spare, cudaStream_t s);
 void ns_grid_carve(Carver& c, int rows, int cols);
 // Waits that ran out since the last call.
 int ns_fused_take_timeouts();

@@ -637,14 +637,14 @@ void ns_grid_carve(Carver& c, int rows, int cols) {
   carve_work(c, Shape(it));
 }
 
-int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, cudaStream_t s) {
+int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, int spare, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
   const uint64_t bit = device_bit();
   if (!(ready.load() & bit)) {
     EGNN_CHECK_CUDA(cudaFuncSetAttribute(ns_grid_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     ready.fetch_or(bit);
   }
-  const int blocks = num_sms_current();
+  const int blocks = std::max(1, num_sms_current() - spare);
   Grid g;
   g.count = 0;
   for (int i = 0; i < b.count; ++i) {
