@@ -10,17 +10,20 @@
 // same block serves as K-major and as MN-major operand.  Products are lo hi +
 // hi lo + hi hi as in the one-block kernel.  At these sizes images stay in L2.
 //
-// A block computes 128 x 128 tiles of its group's products: one warp streams
-// operands through a ring of 64-column stages, one issues the products, sixteen
-// turn accumulators (two, used in turn) into blocks of an image, which leave
-// through shared memory as bulk copies (16-byte stores from the accumulators'
-// rows and the fence behind them took 8,300 cycles a tile, these 6,300).  Blocks
-// of a group meet after each product at a counter in global memory; only the copies
-// of the next product wait for it.  The wait is bounded, and the launch is
+// A block computes tiles of 128 rows and 64 or 128 columns of its group's products:
+// one warp streams operands through a ring of 64-column stages, one issues the
+// products, sixteen turn accumulators (two, used in turn) into blocks of an image,
+// which leave through shared memory as bulk copies (16-byte stores from the
+// accumulators' rows and the fence behind them took 8,300 cycles a tile, these 6,300).
+// Blocks of a group meet after each product at a counter in global memory; only the
+// copies of the next product wait for it.  The wait is bounded, and the launch is
 // cooperative, so all blocks are resident.
 //
-// What bounds it: at one to three tiles a product the chain of copy latency,
-// products, accumulator reads and the meeting, not the tensor cores.
+// What bounds it: the chain of a product, some 13,000 cycles of which the tensor cores
+// work 2,000 to 7,000: meeting and first copies 3,400, the last accumulator's way into
+// shared memory 2,800, from there into L2 3,500.  One 200 x 333 takes 106 us for 5 steps,
+// 30 matrices of H = 256 layers 178 us: 13 GF, three times in half precision, is 24 us
+// of the measured matrix rate.
 //
 // Sums in tensor memory are rounded towards zero at every instruction, by the
 // size of the sum so far.  So lo hi + hi lo has an accumulator of its own, and
@@ -51,21 +54,33 @@ __host__ __device__ inline int up(int a, int b) { return (a + b - 1) / b; }
 struct Work {
   char* x[2];            // images: hi blocks, then lo blocks
   char *a, *b;
-  unsigned* counter;     // arrivals of the group's blocks, for each product
+  unsigned* counter;     // arrivals of the group's blocks, for each phase
+  float* part;           // pieces of A
   double* partial;       // sums of squares of the parts of U
 };
 struct Grid {
   NsItem it[kNsItems];
   Work w[kNsItems];
   int first[kNsItems + 1];   // first block of each matrix's group
-  int count;
+  int count, tile;           // tile: columns of a product that a block computes at once
 };
 constexpr int kParts = 32;   // blocks of a matrix in the norm
 
+// A's sum runs over the long side.  It is split into pieces of at least kSplit chunks
+// of 64 columns, which a group's blocks compute side by side, as float32, and add up,
+// in order, in a phase of its own.  The pieces' number follows from the matrix alone,
+// and with it the result.  In pieces and whole: 64 x 1100 110 and 137 us, 128 x 900 125
+// and 135, 1 x 16384 158 and 848.  From 9 chunks on it is no gain where bands fill the
+// device: 1024 x 1024 305 and 245; pieces of 4 make 30 matrices of 256 x 513 slower
+// (242 and 194), of 9 leave 64 x 1100 at 131.
+constexpr int kSplit = 6, kMostPieces = 64;   // of them all tiles
+
 struct Shape {
   int m, n, m16, n16, bands, xc, ac;   // 128-row bands, 64-column blocks of X and of A
+  int tile;                            // 64 or 128
+  int pieces, piece;                   // of A, and the chunks of each
   bool turn;
-  __host__ __device__ explicit Shape(const NsItem& it) {
+  __host__ __device__ explicit Shape(const NsItem& it, int tile_ = 128) : tile(tile_) {
     turn = it.rows > it.cols;
     m = turn ? it.cols : it.rows;
     n = turn ? it.rows : it.cols;
@@ -74,18 +89,28 @@ struct Shape {
     bands = up(m, 128);
     xc = up(n, 64);
     ac = up(m, 64);
+    pieces = xc / kSplit < kMostPieces / (bands * bands) ? xc / kSplit : kMostPieces / (bands * bands);
+    piece = pieces > 1 ? up(xc, pieces) : xc;
+    pieces = up(xc, piece);
   }
   __host__ __device__ size_t x_bytes() const { return (size_t)bands * xc * kBlk; }   // of hi alone
   __host__ __device__ size_t a_bytes() const { return (size_t)bands * ac * kBlk; }
-  // tiles of a product (0: A, 1: B, 2: X') and its 64-column chunks of K
-  __host__ __device__ int tile_cols(int mode) const { return mode == 2 ? up(n16, 128) : bands; }
-  __host__ __device__ int tiles(int mode) const { return bands * tile_cols(mode); }
-  // rows of a band that hold anything (those a copy moves), and the ring's stages
-  __host__ __device__ int band_rows(int band) const { return m16 - 128 * band < 128 ? m16 - 128 * band : 128; }
-  __host__ __device__ int stage_bytes(int mode) const {
-    const int rows = band_rows(0) * 128;   // a block of the highest band
-    return 2 * rows + (mode == 2 ? 2 * kBlk : bands > 1 ? 2 * rows : 0);
+  __host__ __device__ size_t part_bytes() const { return pieces > 1 ? (size_t)pieces * bands * bands * 65536 : 0; }
+  // Phases of a step: the products 0: A, 1: B, 2: X', and 3: the pieces of A added up.
+  __host__ __device__ int per_step() const { return pieces > 1 ? 4 : 3; }
+  __host__ __device__ int mode(int p) const {
+    const int k = p % per_step();
+    return pieces > 1 && k ? k == 1 ? 3 : k - 1 : k;
   }
+  // tiles of a product
+  __host__ __device__ int tile_cols(int mode) const { return up(mode == 2 ? n16 : m16, tile); }
+  __host__ __device__ int tiles(int mode) const { return bands * tile_cols(mode) * (mode == 0 ? pieces : 1); }
+  // rows of a band that hold anything (those a copy moves), and the ring's stages:
+  // hi and lo of a band of L, then of R
+  __host__ __device__ int band_rows(int band) const { return m16 - 128 * band < 128 ? m16 - 128 * band : 128; }
+  __host__ __device__ int l_bytes() const { return band_rows(0) * 128; }
+  __host__ __device__ int r_bytes(int mode) const { return mode != 2 && bands == 1 ? 0 : tile * 128; }
+  __host__ __device__ int stage_bytes(int mode) const { return 2 * (l_bytes() + r_bytes(mode)); }
   __host__ __device__ int stages(int mode) const {
     const int s = kRing / stage_bytes(mode);
     return s < kMaxStages ? s : kMaxStages;
@@ -112,7 +137,7 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Gr
   const Work& w = g.w[blockIdx.y];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.x == 0)
-    for (int k = threadIdx.x; k < 3 * q.steps; k += 256) w.counter[k] = 0;
+    for (int k = threadIdx.x; k < 4 * q.steps; k += 256) w.counter[k] = 0;
   double ss = 0.0;
   for (Unit u(it.cols, blockIdx.x * 8 + warp, kParts * 8); u.r0 < it.rows; u.next()) {
     float v[8];
@@ -207,6 +232,36 @@ __global__ void __launch_bounds__(256) ns_give_kernel(const __grid_constant__ Gr
   else give<__half>(it, q, sh, hi, lo);
 }
 
+// What the warps of a block need to know of each phase of a step, in shared memory.
+struct Phase {
+  int mode, tn, round, tiles;       // tile columns, tiles of a piece, of all pieces
+  int k16, piece, chunks;           // K in steps of 16; chunks of a piece, and in all
+  int stages, stage_bytes, r_bytes; // the ring
+  __device__ void set(const Shape& sh, int k) {
+    mode = sh.mode(k);
+    tn = sh.tile_cols(mode);
+    round = sh.bands * tn;
+    tiles = sh.tiles(mode);
+    k16 = sh.k16(mode);
+    chunks = up(k16, 4);
+    piece = mode == 0 ? sh.piece : chunks;
+    stages = sh.stages(mode);
+    stage_bytes = sh.stage_bytes(mode);
+    r_bytes = sh.r_bytes(mode);
+  }
+};
+// The t-th tile of a product: its place, and its chunks of K.
+struct Tile {
+  int ti, tj, k0, k1;
+  __device__ __forceinline__ Tile(const Phase& f, int t) {
+    k0 = 0;
+    for (; t >= f.round; t -= f.round) k0 += f.piece;
+    k1 = min(k0 + f.piece, f.chunks);
+    ti = t / f.tn;
+    tj = t - ti * f.tn;
+  }
+};
+
 // ---- the steps ------------------------------------------------------------------
 struct Barriers {
   uint64_t full[kMaxStages], empty[kMaxStages];
@@ -228,30 +283,78 @@ __device__ __forceinline__ void bulk_copy_s2g(void* dst, const void* src, uint32
                : "memory");
 }
 
-// B and X' add a multiple of the same tile of A or X to their product.  That
-// tile comes through the ring anyhow: as two chunks of L (A: columns 2 tj, 2 tj + 1)
-// or of R (X: rows of the band ti), from where the readers take it.
-__device__ __forceinline__ bool old_chunk(int mode, int ti, int tj, int kc) {
-  return mode != 0 && (kc >> 1) == (mode == 1 ? tj : ti);
+// Whether every block of the group has arrived at `counter`; the wait is bounded.
+__device__ __forceinline__ bool wait_group(const unsigned* counter, int group, volatile int* gave_up) {
+  bool here = false;
+  for (uint32_t i = 0; i < (1u << 23) && !here; ++i) {
+    here = load_acquire(counter) == (unsigned)group;
+    if (!here && (i & 255u) == 255u && *gave_up) break;
+  }
+  here = __all_sync(0xffffffffu, here);
+  if (!here) *gave_up = 1;
+  return here;
 }
 
+// B and X' add a multiple of the same tile of A or X to their product.  That
+// tile comes through the ring anyhow: as chunks of L (A: the tile's columns)
+// or of R (X: rows of the band ti), from where the readers take it.
+__device__ __forceinline__ bool old_chunk(int mode, int ti, int tj, int kc, int tile) {
+  return mode == 1 ? kc / (tile >> 6) == tj : mode == 2 && (kc >> 1) == ti;
+}
+
+// Pieces of A: 16 readers' elements of each tile, four columns of a reader's 32 rows after one another.
+__device__ __forceinline__ float4* piece_at(float* part, int tile, int t, int reader) {
+  return reinterpret_cast<float4*>(part) + ((size_t)t * kReaders + reader) * (2 * tile) + (threadIdx.x & 31);
+}
+// A (hi; lo `size` bytes further) from its pieces, eight columns of a reader's rows at a time.
+template <int tile>
+__device__ __noinline__ void add_pieces(float* part, char* a, size_t size, int tn, int tiles, int pieces, int m16, int blocks,
+                                        int first, int stride) {
+  constexpr int W = tile / 4, units = W / 8;   // of a reader
+#pragma unroll 1
+  for (int u = first; u < tiles * kReaders * units; u += stride) {
+    const int at = u / units, t = at / kReaders, reader = at % kReaders;
+    // a reader is a warp, of which the first two do not read: its rows follow from the warp
+    const int row = (reader + 2 & 3) * 32 + (threadIdx.x & 31);
+    const int c = tile * (t % tn) + (reader >> 2) * W + u % units * 8;
+    if (c >= m16) continue;
+    const float4* from = piece_at(part, tile, t, reader) + u % units * 64;
+    float v[8] = {};
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k, from += tiles * kReaders * 2 * tile) {
+      const float4 x = __ldcg(from), y = __ldcg(from + 32);
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split2(v[2 * k], v[2 * k + 1], h[k], l[k]);
+    char* const to = a + (size_t)(t / tn) * blocks * kBlk + sw128_offset(row, c, 128);
+    *reinterpret_cast<uint4*>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(to + size) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+}
+
+template <int tile>   // columns of a product that a block computes at once: 64 or 128
 __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_constant__ Grid g,
                                                               const __grid_constant__ NsScalars q) {
   extern __shared__ char raw[];
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_s;
+  __shared__ Phase phase[4];
   __shared__ int gave_up_s;
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   int item = 0;
   while (item + 1 < g.count && g.first[item + 1] <= (int)blockIdx.x) ++item;
-  const Shape sh(g.it[item]);
+  const Shape sh(g.it[item], tile);
   const Work& w = g.w[item];
   const int group = g.first[item + 1] - g.first[item], rank = blockIdx.x - g.first[item];
   char* const ring = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
   char* const out = ring + kRing;
   volatile int* const gave_up = &gave_up_s;
 
+  if (warp == 0 && lane < sh.per_step()) phase[lane].set(sh, lane);
   if (warp == 1) {
     tmem_alloc(&tmem_s, 512);
     if (lane == 0) {
@@ -275,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = tmem_s;
-  const int phases = 3 * q.steps, segment = sh.segment();
+  const int per_step = sh.per_step(), phases = per_step * q.steps, segment = sh.segment(), l_all = sh.l_bytes();
   bool ok = true;
 
   if (warp == 0) {
@@ -284,45 +387,39 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     uint32_t used = 0, parity = 0;   // bit k: stage k has been filled; the parity of its last filling
     uint32_t old = 0, old_parity = 0;   // the same of its fillings with a chunk that the readers take from
 #pragma unroll 1
-    for (int p = 0; p < phases && ok; ++p) {
-      const int mode = p % 3, cur = (p / 3) & 1;
-      if (p > 0) {   // every block of the group has written its tiles of the last product
-        bool here = false;
-        for (uint32_t i = 0; i < (1u << 23) && !here; ++i) {
-          here = load_acquire(w.counter + p - 1) == (unsigned)group;
-          if (!here && (i & 255u) == 255u && *gave_up) break;
-        }
-        here = __all_sync(0xffffffffu, here);
-        if (!here) {
-          *gave_up = 1;
-          ok = false;
-          break;
-        }
+    for (int p = 0, k = 0, cur = 0; p < phases && ok; ++p, ++k) {
+      if (k == per_step) k = 0, cur ^= 1;
+      const Phase& f = phase[k];
+      const int mode = f.mode;
+      if (mode == 3) continue;
+      if (p > 0) {   // every block of the group has written its tiles of the last phase
+        if (!(ok = wait_group(w.counter + p - 1, group, gave_up))) break;
         fence_proxy_async_all();
       }
       const char* Lh = mode == 0 ? w.x[cur] : mode == 1 ? w.a : w.b;
       const char* Rh = mode == 1 ? w.a : w.x[cur];
       const size_t lsize = mode == 0 ? sh.x_bytes() : sh.a_bytes(), rsize = mode == 1 ? sh.a_bytes() : sh.x_bytes();
       const int lc = mode == 0 ? sh.xc : sh.ac;   // column blocks of L (and of a K-major R)
-      const int chunks = up(sh.k16(mode), 4), tn = sh.tile_cols(mode);
-      const int stages = sh.stages(mode), stage_bytes = sh.stage_bytes(mode), full_rows = sh.band_rows(0) * 128;
+      const int stages = f.stages, stage_bytes = f.stage_bytes, r_all = f.r_bytes;
       int st = 0;
 #pragma unroll 1
-      for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
-        const int ti = t / tn, tj = t % tn;
-        const int rcols = mode == 2 ? min(2, sh.xc - 2 * tj) : 0;   // 64-column blocks of an MN-major R
-        const bool shared = mode != 2 && ti == tj;
-        const uint32_t lbytes = sh.band_rows(ti) * 128, rbytes = mode == 2 || shared ? 0 : sh.band_rows(tj) * 128;
+      for (int t = rank; t < f.tiles && ok; t += group) {
+        const Tile at(f, t);
+        const int ti = at.ti, tj = at.tj;
+        const int rcols = mode == 2 ? min(tile >> 6, sh.xc - (tile >> 6) * tj) : 0;   // 64-column blocks of an MN-major R
+        const int rrow = tile * tj & 127;                                             // first row in its band of a K-major R
+        const bool shared = mode != 2 && ti == tile * tj >> 7;
+        const uint32_t lbytes = sh.band_rows(ti) * 128, rbytes = mode == 2 || shared ? 0 : min(tile, sh.m16 - tile * tj) * 128;
         const uint32_t bytes = 2 * lbytes + 2 * rbytes + rcols * kBlk;
 #pragma unroll 1
-        for (int kc = 0; kc < chunks && ok; ++kc) {
+        for (int kc = at.k0; kc < at.k1 && ok; ++kc) {
           if ((used >> st & 1u) && !(ok = wait_bar(&bar.empty[st], parity >> st & 1u, gave_up))) break;
           if (old >> st & 1u) {
             if (!(ok = wait_bar(&bar.old_read[st], old_parity >> st & 1u, gave_up))) break;
             old &= ~(1u << st);
             old_parity ^= 1u << st;
           }
-          if (old_chunk(mode, ti, tj, kc)) old |= 1u << st;
+          if (old_chunk(mode, ti, tj, kc, tile)) old |= 1u << st;
           if (used >> st & 1u) parity ^= 1u << st;
           used |= 1u << st;
           if (lane == 0) {
@@ -330,18 +427,18 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
             const size_t l = (size_t)(ti * lc + kc) * kBlk;
             mbar_expect_tx_bytes(&bar.full[st], bytes);
             bulk_copy_g2s(to, Lh + l, lbytes, &bar.full[st]);
-            bulk_copy_g2s(to + full_rows, Lh + lsize + l, lbytes, &bar.full[st]);
-            char* const rt = to + 2 * full_rows;
+            bulk_copy_g2s(to + l_all, Lh + lsize + l, lbytes, &bar.full[st]);
+            char* const rt = to + 2 * l_all;
             if (mode == 2) {   // 64 rows of X: half of a block for each column block
               for (int c = 0; c < rcols; ++c) {
-                const size_t r = (size_t)((kc >> 1) * sh.xc + 2 * tj + c) * kBlk + (kc & 1) * (kBlk / 2);
+                const size_t r = (size_t)((kc >> 1) * sh.xc + (tile >> 6) * tj + c) * kBlk + (kc & 1) * (kBlk / 2);
                 bulk_copy_g2s(rt + c * (kBlk / 2), Rh + r, kBlk / 2, &bar.full[st]);
-                bulk_copy_g2s(rt + kBlk + c * (kBlk / 2), Rh + rsize + r, kBlk / 2, &bar.full[st]);
+                bulk_copy_g2s(rt + r_all + c * (kBlk / 2), Rh + rsize + r, kBlk / 2, &bar.full[st]);
               }
             } else if (!shared) {
-              const size_t r = (size_t)(tj * lc + kc) * kBlk;
+              const size_t r = (size_t)((tile * tj >> 7) * lc + kc) * kBlk + rrow * 128;
               bulk_copy_g2s(rt, Rh + r, rbytes, &bar.full[st]);
-              bulk_copy_g2s(rt + full_rows, Rh + rsize + r, rbytes, &bar.full[st]);
+              bulk_copy_g2s(rt + r_all, Rh + rsize + r, rbytes, &bar.full[st]);
             }
           }
           if (++st == stages) st = 0;
@@ -359,27 +456,32 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     int seg = 0;
     uint32_t parity = 0;   // of each stage's next filling
 #pragma unroll 1
-    for (int p = 0; p < phases && ok; ++p) {
-      const int mode = p % 3, tn = sh.tile_cols(mode), k16 = sh.k16(mode), chunks = up(k16, 4);
-      const int stages = sh.stages(mode), stage_bytes = sh.stage_bytes(mode), full_rows = sh.band_rows(0) * 128;
+    for (int p = 0, k = 0; p < phases && ok; ++p, ++k) {
+      if (k == per_step) k = 0;
+      const Phase& f = phase[k];
+      const int mode = f.mode, k16 = f.k16;
+      if (mode == 3) continue;
+      const int stages = f.stages, stage_bytes = f.stage_bytes, r_all = f.r_bytes;
       int st = 0;
 #pragma unroll 1
-      for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
-        const int ti = t / tn, tj = t % tn;
-        const bool shared = mode != 2 && ti == tj;
-        const uint32_t idesc = make_idesc_f16(128, min(128, (mode == 2 ? sh.n16 : sh.m16) - 128 * tj), 0, mode == 2);
+      for (int t = rank; t < f.tiles && ok; t += group) {
+        const Tile x(f, t);
+        const int ti = x.ti, tj = x.tj;
+        const bool shared = mode != 2 && ti == tile * tj >> 7;
+        const uint32_t idesc = make_idesc_f16(128, min(tile, (mode == 2 ? sh.n16 : sh.m16) - tile * tj), 0, mode == 2);
 #pragma unroll 1
-        for (int kc = 0; kc < chunks && ok; ++kc) {
-          const bool start = kc % segment == 0;
+        for (int kc = x.k0; kc < x.k1 && ok; ++kc) {
+          const bool start = (kc - x.k0) % segment == 0;
           // the accumulator's last user has been read
           if (start && !(ok = wait_bar(&bar.acc_empty[seg & 1], ((seg >> 1) & 1) ^ 1, gave_up))) break;
           if (!(ok = wait_bar(&bar.full[st], parity >> st & 1u, gave_up))) break;
           parity ^= 1u << st;
           const uint32_t d = tmem + (seg & 1) * 256;   // hi hi, and the small terms 128 columns further
-          const uint32_t at = smem_u32(ring + st * stage_bytes), rt = shared ? at : at + 2 * full_rows;
-          const uint64_t lh = make_desc(at, 16, 1024), ll = make_desc(at + full_rows, 16, 1024);
-          const uint64_t rh = mode == 2 ? make_desc(rt, kBlk / 2, 1024) : make_desc(rt, 16, 1024);
-          const uint64_t rl = mode == 2 ? make_desc(rt + kBlk, kBlk / 2, 1024) : make_desc(rt + full_rows, 16, 1024);
+          // a K-major R of the band ti is part of L
+          const uint32_t at = smem_u32(ring + st * stage_bytes), rt = shared ? at + (tile * tj & 127) * 128 : at + 2 * l_all;
+          const uint32_t rlo = rt + (shared ? l_all : r_all), lbo = mode == 2 ? kBlk / 2 : 16;
+          const uint64_t lh = make_desc(at, 16, 1024), ll = make_desc(at + l_all, 16, 1024);
+          const uint64_t rh = make_desc(rt, lbo, 1024), rl = make_desc(rlo, lbo, 1024);
           const int nk = k16 - 4 * kc;
           const uint32_t rstep = mode == 2 ? 128 : 2;
 #pragma unroll
@@ -391,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
                                 idesc, !(start && pr != 1 && j == 0));
           if (one) mma_commit(&bar.empty[st]);
           if (++st == stages) st = 0;
-          if ((kc + 1) % segment == 0 || kc + 1 == chunks) {
+          if ((kc + 1 - x.k0) % segment == 0 || kc + 1 == x.k1) {
             if (one) mma_commit(&bar.acc_full[seg & 1]);
             ++seg;
           }
@@ -403,18 +505,28 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     wait_bar(&bar.drained, 0, gave_up);
   } else {
     // ---- accumulators into images: warp w reads the rows 32 (w % 4) .. + 31 of
-    // one 32-column piece
-    const int row = (warp & 3) * 32 + lane, c = ((warp - 2) >> 2) * 32;
+    // a quarter of the tile's columns
+    constexpr int W = tile / 4;
+    const int row = (warp & 3) * 32 + lane, c = ((warp - 2) >> 2) * W, c16 = c >> 4 & 1;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const float loss = ns_mean_loss(4 * segment);
-    int seg = 0, outs = 0, frees = 0;
+    int seg = 0, outs = 0, sent = 0;
     uint32_t parity = 0;   // of each stage's next filling
 #pragma unroll 1
-    for (int p = 0; p < phases && ok; ++p) {
-      const int mode = p % 3, cur = (p / 3) & 1, tn = sh.tile_cols(mode), chunks = up(sh.k16(mode), 4);
+    for (int p = 0, phase_of_step = 0, cur = 0; p < phases && ok; ++p, ++phase_of_step) {
+      if (phase_of_step == per_step) phase_of_step = 0, cur ^= 1;
+      const Phase& f = phase[phase_of_step];
+      const int mode = f.mode;
+      if (mode == 3) {
+        if (!(ok = wait_group(w.counter + p - 1, group, gave_up))) break;
+        add_pieces<tile>(w.part, w.a, sh.a_bytes(), phase[0].tn, phase[0].round, sh.pieces, sh.m16, sh.ac,
+                         rank + group * (warp - 2), group * kReaders);
+        fence_proxy_async_all();
+      }
+      const bool apart = mode == 0 && sh.pieces > 1;
       const int blocks = mode == 2 ? sh.xc : sh.ac;
       const size_t size = mode == 2 ? sh.x_bytes() : sh.a_bytes();
-      const int stages = sh.stages(mode), stage_bytes = sh.stage_bytes(mode), full_rows = sh.band_rows(0) * 128;
+      const int stages = f.stages, stage_bytes = f.stage_bytes, r_all = f.r_bytes;
       int st = 0;
       char* const dst = mode == 0 ? w.a : mode == 1 ? w.b : w.x[cur ^ 1];
       const bool last = p + 1 == phases;   // X' itself, not scaled
@@ -423,43 +535,48 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
       const float wp = mode == 0 ? q.sa / (q.sx * q.sx) : mode == 1 ? q.c * q.sb / (q.sa * q.sa) : end / q.sb;
       const float wo = mode == 1 ? q.b * q.sb / q.sa : q.a * end;
 #pragma unroll 1
-      for (int t = rank; t < sh.tiles(mode) && ok; t += group) {
-        const int ti = t / tn, tj = t % tn;
-        const int N = min(128, (mode == 2 ? sh.n16 : sh.m16) - 128 * tj);
+      for (int t = rank; mode != 3 && t < f.tiles && ok; t += group) {
+        const Tile at(f, t);
+        const int ti = at.ti, tj = at.tj;
+        const int N = min(tile, (mode == 2 ? sh.n16 : sh.m16) - tile * tj);
         const bool here = c < N;
         const size_t band = (size_t)ti * blocks * kBlk;
-        float acc[32];
+        float acc[W];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) acc[k] = 0.f;
-        const int mine = mode == 1 ? 2 * tj + (c >> 6) : 2 * ti + (row >> 6);   // the chunk with this warp's part
+        for (int k = 0; k < W; ++k) acc[k] = 0.f;
+        const int mine = mode == 1 ? (tile * tj + c) >> 6 : 2 * ti + (row >> 6);   // the chunk with this warp's part
 #pragma unroll 1
-        for (int kc = 0; kc < chunks; ++kc) {
-          if (old_chunk(mode, ti, tj, kc)) {
+        for (int kc = at.k0; kc < at.k1; ++kc) {
+          if (old_chunk(mode, ti, tj, kc, tile)) {
             if (here && kc == mine) {
               if (!(ok = wait_bar(&bar.full[st], parity >> st & 1u, gave_up))) break;
               const uint32_t stage = smem_u32(ring) + st * stage_bytes;
               const uint32_t from = mode == 1 ? row_at(stage, 128, row, c & 63)
-                                              : row_at(stage + 2 * full_rows + (c >> 6) * (kBlk / 2), 128, row & 63, c & 63);
-              float x[32];
-              load_pairs32(from, from + (mode == 1 ? full_rows : kBlk), x);
+                                              : row_at(stage + 2 * l_all + (c >> 6) * (kBlk / 2), 128, row & 63, c & 63);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) acc[k] = fmaf(wo, x[k], acc[k]);
+              for (int h = 0; h < W; h += 16) {
+                float x[16];
+                load_pairs16(from, from + (mode == 1 ? l_all : r_all), c16 + (h >> 4), x);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) acc[h + k] = fmaf(wo, x[k], acc[h + k]);
+              }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.old_read[st]);
           }
           parity ^= 1u << st;
           if (++st == stages) st = 0;
-          if ((kc + 1) % segment && kc + 1 < chunks) continue;
+          if ((kc + 1 - at.k0) % segment && kc + 1 < at.k1) continue;
           if (!(ok = wait_bar(&bar.acc_full[seg & 1], (seg >> 1) & 1, gave_up, q.wait_polls))) break;
           if (here) {
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {   // small terms and hi hi, 16 columns each
-              float v[16];
-              tmem_ld16(tmem + (seg & 1) * 256 + (h & 1 ? 0 : 128) + lanes + c + (h >> 1) * 16, v);
-              const float l = h & 1 ? loss : 0.f;
+            for (int h = 0; h < W; h += 16) {
+              float small[16], v[16];
+              const uint32_t at16 = tmem + (seg & 1) * 256 + lanes + c + h;
+              tmem_ld16x2(at16 + 128, at16, small, v);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) acc[(h >> 1) * 16 + k] = fmaf(wp, fmaf(v[k], l, v[k]), acc[(h >> 1) * 16 + k]);
+              for (int k = 0; k < 16; ++k)
+                acc[h + k] = fmaf(wp, fmaf(v[k], loss, v[k]), fmaf(wp, small[k], acc[h + k]));
             }
           }
           fence_before_sync();
@@ -468,24 +585,19 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           ++seg;
         }
         if (!ok) break;
-        // The block's last tile of the product leaves through the ring, which is
-        // idle until the group has met, hi and lo at once; others, while the ring
-        // serves the next tile, through the two blocks behind it, one after the other.
-        const uint32_t bytes = sh.band_rows(ti) * 128;
-        const bool ring_free = t + group >= sh.tiles(mode);
-        uint32_t words[2][16];   // hi and lo of 32 columns; at the end float32 columns 0 .. 15 and 16 .. 31
-        auto write = [&](char* at, int part) {
-          if (!here) return;
-          const uint32_t to = row_at(smem_u32(at), 128, row, c);
+        if (apart) {
+          if (here) {
+            float4* const to = piece_at(w.part, tile, t, warp - 2);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            sts16(to ^ (j << 4), words[part][4 * j], words[part][4 * j + 1], words[part][4 * j + 2], words[part][4 * j + 3]);
-        };
-        auto meet = [&]() {   // of the readers
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.written);
-          return wait_bar(&bar.written, outs++, gave_up);
-        };
+            for (int k = 0; k < W / 4; ++k) to[32 * k] = make_float4(acc[4 * k], acc[4 * k + 1], acc[4 * k + 2], acc[4 * k + 3]);
+          }
+          continue;
+        }
+        // A tile leaves as hi and lo through the blocks behind the ring.  They hold one of
+        // two 128 columns wide: those go one after the other, but for the block's last
+        // tile of the product, which takes the ring, idle until the group has met.
+        const uint32_t bytes = sh.band_rows(ti) * 128;
+        const bool ring_free = t + group >= f.tiles;
         auto hand_on = [&]() {   // true in warp 2 when all have written
           fence_proxy_async();
           __syncwarp();
@@ -494,42 +606,69 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
           ++outs;
           return warp == 2 && ok;
         };
+        auto out_free = [&]() {   // the copies out of the blocks behind the ring have read them
+          if (sent) {
+            if (warp == 2 && lane == 0) {
+              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              mbar_arrive(&bar.out_free);
+            }
+            __syncwarp();
+            ok = wait_bar(&bar.out_free, sent - 1, gave_up);
+          }
+          ++sent;
+          return ok;
+        };
         auto send = [&](char* from, int part) {
-          char* const to = dst + part * size + band + (size_t)2 * tj * kBlk;
+          char* const to = dst + part * size + band + (size_t)(tile * tj >> 6) * kBlk;
           bulk_copy_s2g(to, from, bytes);
           if (N > 64) bulk_copy_s2g(to + kBlk, from + kBlk, bytes);
         };
+        auto commit = []() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); };
         auto emit = [&]() {
-          if (last) {
+          if (tile == 64 || ring_free) {
+            if (tile == 64) {
+              if (!out_free()) return;
+            } else if (mode != 0) {   // every reader has taken its part of the old tile out of the ring
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bar.written);
+              if (!(ok = wait_bar(&bar.written, outs++, gave_up))) return;
+            }
+            char* const from = tile == 64 ? out : ring;
+            if (here) {
+              const uint32_t hi = row_at(smem_u32(from), 128, row, c), lo = hi + tile * 256;
 #pragma unroll
-            for (int k = 0; k < 32; ++k) words[k >> 4][k & 15] = __float_as_uint(acc[k]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) split2(acc[2 * k], acc[2 * k + 1], words[0][k], words[1][k]);
-          }
-          if (ring_free) {
-            // every reader has taken its part of the old tile out of the ring
-            if (mode != 0 && !(ok = meet())) return;
-            write(ring, 0);
-            write(ring + 2 * kBlk, 1);
+              for (int h = 0; h < W; h += 16)
+                if (last) store_raw16(hi, lo, c16 + (h >> 4), acc + h);
+                else store_pairs16(hi, lo, c16 + (h >> 4), acc + h);
+            }
             if (hand_on() && lane == 0) {
-              send(ring, 0);
-              send(ring + 2 * kBlk, 1);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              send(from, 0);
+              send(from + tile * 256, 1);
+              commit();
             }
             __syncwarp();
             return;
           }
+          uint32_t words[2][W / 2];   // hi and lo; at the end float32 columns 0 .. 15 and 16 .. 31
+          if (last) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) words[2 * k / W][k % (W / 2)] = __float_as_uint(acc[k]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < W / 2; ++k) split2(acc[2 * k], acc[2 * k + 1], words[0][k], words[1][k]);
+          }
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
-            if (frees && !(ok = wait_bar(&bar.out_free, frees - 1, gave_up))) return;
-            ++frees;
-            write(out, part);
+            if (!out_free()) return;
+            if (here) {
+              const uint32_t to = row_at(smem_u32(out), 128, row, c);
+#pragma unroll
+              for (int j = 0; j < W / 8; ++j)
+                sts16(to ^ (j << 4), words[part][4 * j], words[part][4 * j + 1], words[part][4 * j + 2], words[part][4 * j + 3]);
+            }
             if (hand_on() && lane == 0) {
               send(out, part);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-              mbar_arrive(&bar.out_free);
+              commit();
             }
             __syncwarp();
           }
@@ -538,6 +677,12 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
         if (!ok) break;
       }
       if (!ok) break;
+      if (apart || mode == 3) {   // what all readers have stored
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.written);
+        if (warp == 2 && !(ok = wait_bar(&bar.written, outs, gave_up))) break;
+        ++outs;
+      }
       if (warp == 2 && lane == 0) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         fence_proxy_async_all();
@@ -556,34 +701,54 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   }
 }
 
-// The time of a matrix's step with a group of g blocks, in chunks of K.
+// The time of a matrix's step with a group of g blocks, in cycles, fitted to lists of
+// 200 x 333 and 256 x 513: a phase's meeting and first copies, and for each tile of a
+// block its chunks of K and its way out.
 int step_time(const Shape& s, int g) {
+  const int tile = s.tile == 64 ? 5000 : 5500, chunk = s.tile == 64 ? 550 : 1000;
   int t = 0;
-  for (int mode = 0; mode < 3; ++mode) t += up(s.tiles(mode), g) * up(s.k16(mode), 4);
+  for (int mode = 0; mode < 3; ++mode)
+    t += 8000 + 30 * g + up(s.tiles(mode), g) * (tile + chunk * (mode == 0 ? s.piece : up(s.k16(mode), 4)));
   return t;
 }
 
-// Shares `blocks` out: again and again to the matrix that takes longest, as
-// many more as shorten its step.
-void share_out(Grid& g, int blocks) {
-  int size[kNsItems], time[kNsItems], left = blocks - g.count;
+// Shares `blocks` out, size[i] to matrix i: again and again to the matrix that takes
+// longest, as many more as shorten its step.  Returns the longest step's time.
+int allot(const Grid& g, int blocks, int tile, int* size) {
+  int time[kNsItems], left = blocks - g.count, most = 0;
+  bool done[kNsItems] = {};
   for (int i = 0; i < g.count; ++i) {
     size[i] = 1;
-    time[i] = step_time(Shape(g.it[i]), 1);
+    time[i] = step_time(Shape(g.it[i], tile), 1);
   }
   while (left > 0) {
-    int worst = 0;
-    for (int i = 1; i < g.count; ++i)
-      if (time[i] > time[worst]) worst = i;
-    const Shape s(g.it[worst]);
-    const int most = std::min(size[worst] + left, std::max(s.tiles(0), s.tiles(2)));
-    int next = size[worst] + 1;
-    while (next <= most && step_time(s, next) >= time[worst]) ++next;
-    if (next > most) break;
+    int worst = -1;
+    for (int i = 0; i < g.count; ++i)
+      if (!done[i] && (worst < 0 || time[i] > time[worst])) worst = i;
+    if (worst < 0) break;
+    const Shape s(g.it[worst], tile);
+    const int end = std::min(size[worst] + left, std::max(s.tiles(0), s.tiles(2)));
+    int next = size[worst] + 1, t = 0;
+    while (next <= end && (t = step_time(s, next)) >= time[worst]) ++next;
+    if (next > end) {
+      done[worst] = true;
+      continue;
+    }
     left -= next - size[worst];
     size[worst] = next;
-    time[worst] = step_time(s, next);
+    time[worst] = t;
   }
+  for (int i = 0; i < g.count; ++i) most = std::max(most, time[i]);
+  return most;
+}
+
+// Tiles 64 or 128 columns wide, whichever let the longest step end first: 64 make more
+// of them, each sooner done.  64 and 128: 200 x 333 110 and 130 us, 16 matrices of 256 x 513
+// 153 and 180, 30 of them 208 and 179.
+void share_out(Grid& g, int blocks) {
+  int size64[kNsItems], size128[kNsItems];
+  g.tile = allot(g, blocks, 64, size64) < allot(g, blocks, 128, size128) ? 64 : 128;
+  const int* const size = g.tile == 64 ? size64 : size128;
   g.first[0] = 0;
   for (int i = 0; i < g.count; ++i) g.first[i + 1] = g.first[i] + size[i];
 }
@@ -595,7 +760,8 @@ Work carve_work(Carver& c, const Shape& s) {
   w.a = c.take<char>(2 * s.a_bytes());
   w.b = c.take<char>(2 * s.a_bytes());
   w.partial = c.take<double>(kParts);
-  w.counter = c.take<unsigned>(3 * kNsMaxSteps);
+  w.counter = c.take<unsigned>(4 * kNsMaxSteps);
+  w.part = c.take<float>(s.part_bytes() / 4);
   return w;
 }
 
@@ -620,7 +786,7 @@ int run(Grid& g, const NsScalars& q, int blocks, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    EGNN_CHECK_CUDA(cudaLaunchKernelEx(&cfg, ns_grid_kernel, (const Grid&)g, q));
+    EGNN_CHECK_CUDA(cudaLaunchKernelEx(&cfg, g.tile == 64 ? ns_grid_kernel<64> : ns_grid_kernel<128>, (const Grid&)g, q));
     EGNN_CHECK_LAUNCH();
   }
   EGNN_CHECK_CUDA(launch_pdl(ns_give_kernel, grid, dim3(256), 0, s, g, q));
@@ -641,7 +807,8 @@ int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, int spare, cudaStre
   static std::atomic<uint64_t> ready{0};
   const uint64_t bit = device_bit();
   if (!(ready.load() & bit)) {
-    EGNN_CHECK_CUDA(cudaFuncSetAttribute(ns_grid_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    EGNN_CHECK_CUDA(cudaFuncSetAttribute(ns_grid_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
+    EGNN_CHECK_CUDA(cudaFuncSetAttribute(ns_grid_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
     ready.fetch_or(bit);
   }
   const int blocks = std::max(1, num_sms_current() - spare);

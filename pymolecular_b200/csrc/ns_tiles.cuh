@@ -56,10 +56,11 @@ __device__ __forceinline__ void store_pairs16(uint32_t hi, uint32_t lo, int half
     sts16(lo ^ chunk, l[0], l[1], l[2], l[3]);
   }
 }
-__device__ __forceinline__ void load_pairs32(uint32_t hi, uint32_t lo, float (&v)[32]) {
+__device__ __forceinline__ void load_pairs16(uint32_t hi, uint32_t lo, int half, float* v) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint4 h = lds16(hi ^ (j << 4)), l = lds16(lo ^ (j << 4));
+  for (int j = 0; j < 2; ++j) {
+    const uint32_t chunk = (2 * half + j) << 4;
+    const uint4 h = lds16(hi ^ chunk), l = lds16(lo ^ chunk);
     const uint32_t hh[4] = {h.x, h.y, h.z, h.w}, ll[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -67,6 +68,10 @@ __device__ __forceinline__ void load_pairs32(uint32_t hi, uint32_t lo, float (&v
       v[8 * j + 2 * k + 1] = add_high(hh[k], add_high(ll[k], 0.f));
     }
   }
+}
+__device__ __forceinline__ void load_pairs32(uint32_t hi, uint32_t lo, float (&v)[32]) {
+  load_pairs16(hi, lo, 0, v);
+  load_pairs16(hi, lo, 1, v + 16);
 }
 // Columns 16 half .. + 15 as float32.
 __device__ __forceinline__ void store_raw16(uint32_t hi, uint32_t lo, int half, const float* v) {

@@ -82,6 +82,19 @@ def test_largest_sides(cuda_device):
         _check(G, orthogonalize(G))
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 767), (1, 769), (17, 5000), (100, 769), (2000, 65), (130, 770), (1555, 129), (257, 2100), (600, 4000)])
+def test_long_sums_in_pieces(rows, cols, cuda_device):
+    """Matrices whose A = X X^T is computed in pieces of its long sum, and the
+    same result in a list, where other groups of blocks share them out."""
+    g = torch.Generator(device="cuda").manual_seed(16)
+    G = _gradient(rows, cols, g)
+    one = orthogonalize(G)
+    _check(G, one)
+    others = [_gradient(200, 300, g) for _ in range(40)]
+    assert torch.equal(orthogonalize([*others[:7], G])[7], one)
+    assert torch.equal(orthogonalize([G, *others])[0], one)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_lists_batches_and_strides(dtype, cuda_device):
     """One call over matrices of many sizes gives each what a call of its own
