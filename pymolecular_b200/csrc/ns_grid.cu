@@ -58,10 +58,11 @@ struct Work {
   float* part;           // pieces of A
   double* partial;       // sums of squares of the parts of U
 };
+constexpr int kItems = 64;   // matrices of one launch
 struct Grid {
-  NsItem it[kNsItems];
-  Work w[kNsItems];
-  int first[kNsItems + 1];   // first block of each matrix's group
+  NsItem it[kItems];
+  Work w[kItems];
+  int first[kItems + 1];   // first block of each matrix's group
   int count, tile;           // tile: columns of a product that a block computes at once
 };
 constexpr int kParts = 32;   // blocks of a matrix in the norm
@@ -715,8 +716,8 @@ int step_time(const Shape& s, int g) {
 // Shares `blocks` out, size[i] to matrix i: again and again to the matrix that takes
 // longest, as many more as shorten its step.  Returns the longest step's time.
 int allot(const Grid& g, int blocks, int tile, int* size) {
-  int time[kNsItems], left = blocks - g.count, most = 0;
-  bool done[kNsItems] = {};
+  int time[kItems], left = blocks - g.count, most = 0;
+  bool done[kItems] = {};
   for (int i = 0; i < g.count; ++i) {
     size[i] = 1;
     time[i] = step_time(Shape(g.it[i], tile), 1);
@@ -746,7 +747,7 @@ int allot(const Grid& g, int blocks, int tile, int* size) {
 // of them, each sooner done.  64 and 128: 200 x 333 110 and 130 us, 16 matrices of 256 x 513
 // 153 and 180, 30 of them 208 and 179.
 void share_out(Grid& g, int blocks) {
-  int size64[kNsItems], size128[kNsItems];
+  int size64[kItems], size128[kItems];
   g.tile = allot(g, blocks, 64, size64) < allot(g, blocks, 128, size128) ? 64 : 128;
   const int* const size = g.tile == 64 ? size64 : size128;
   g.first[0] = 0;
@@ -817,7 +818,7 @@ int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, int spare, cudaStre
   for (int i = 0; i < b.count; ++i) {
     g.it[g.count] = b.it[i];
     g.w[g.count] = carve_work(c, Shape(b.it[i]));
-    if (++g.count == std::min(kNsItems, blocks) || i + 1 == b.count) {
+    if (++g.count == std::min(kItems, blocks) || i + 1 == b.count) {
       EGNN_TRY(run(g, q, blocks, s));
       g.count = 0;
     }

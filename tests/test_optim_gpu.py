@@ -374,6 +374,15 @@ def test_many_matrices_and_two_graphs_that_share_a_pool(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(outs[k], want[2 * k:2 * k + 2]))
 
 
+def test_more_small_matrices_than_a_batch_holds(cuda_device):
+    g = torch.Generator(device="cuda").manual_seed(17)
+    mats = [_gradient(9 + k % 5, 20, g) for k in range(333)] + [_gradient(140, 150, g)]
+    got = orthogonalize(mats)
+    for k in (0, 159, 160, 161, 319, 320, 332, 333):
+        assert torch.equal(got[k], orthogonalize(mats[k]))
+    _check(mats[200], got[200])
+
+
 def test_rows_far_apart_and_an_offset_past_32_bits(cuda_device):
     """Row strides that put a matrix over more than 4 GB."""
     g = torch.Generator(device="cuda").manual_seed(14)
