@@ -13,7 +13,7 @@
 // global memory sees the matrix once on the way in and once on the way out.
 // The same X tile is the K-major operand of X X^T and the MN-major operand of
 // B X.  Shared memory bounds the blocks of 64 columns of X and A to 7 for m > 64
-// and 14 for m > 32, tensor memory n to 1024.
+// and 13 for m > 32, tensor memory n to 1024.
 //
 // What bounds it: a chain of three dependent products a step, on one SM.  A step of
 // 128 x 257 takes 15,000 cycles, its products alone 8,300 (three half-precision
