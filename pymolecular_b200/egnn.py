@@ -250,6 +250,8 @@ class E_GCL(nn.Module):
 class EGNN(nn.Module):
     """EGNN model (egnn_clean.py:106-146): embedding_in, n_layers E_GCL, embedding_out."""
 
+    node_norm = False   # also of models that were pickled before there were norms
+
     def __init__(self, in_node_nf, hidden_nf, out_node_nf, in_edge_nf=0, device='cpu',
                  act_fn=nn.SiLU(), n_layers=4, residual=True, attention=False, normalize=False,
                  tanh=False, precision: str = "fp32", node_norm: bool = False):

@@ -40,7 +40,9 @@ def _options(steps, a, b, c, eps):
 
 def _workspace(sizes: Sequence[int], device) -> Tuple[torch.Tensor, int]:
     """sizes: rows, cols of each matrix in turn."""
-    nbytes = nat.lib().egnn_orthogonalize_workspace_size(len(sizes) // 2, struct.pack("%di" % len(sizes), *sizes))
+    nbytes = 0
+    if max(sizes) < 1 << 31:
+        nbytes = nat.lib().egnn_orthogonalize_workspace_size(len(sizes) // 2, struct.pack("%di" % len(sizes), *sizes))
     if not nbytes:
         raise ValueError("matrices have at most 16384 rows and columns, and the smaller side at most 1024")
     return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes

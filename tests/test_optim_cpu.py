@@ -9,7 +9,7 @@ from torch import nn
 
 from conftest import ROOT
 from pymolecular_b200 import EGNN, Muon, layer_norm, muon_step, orthogonalize
-from pymolecular_b200 import _native as nat
+from pymolecular_b200 import _native as nat, optim
 from pymolecular_b200.optim import COEFFICIENTS
 
 BAD, UNSUPPORTED, WORKSPACE = nat.EGNN_ERR_INVALID_ARG, nat.EGNN_ERR_UNSUPPORTED, nat.EGNN_ERR_WORKSPACE
@@ -157,3 +157,15 @@ def test_node_norm_keeps_the_other_parameters():
     normed = EGNN(5, 32, 1, n_layers=2, node_norm=True).state_dict()
     assert set(normed) - set(plain) == {f"norm_{i}.{n}" for i in range(2) for n in ("weight", "bias")}
     assert all(torch.equal(v, normed[k]) for k, v in plain.items())
+
+
+def test_models_from_before_there_were_norms():
+    model = EGNN(2, 32, 1, n_layers=1)
+    del model.__dict__["node_norm"]   # as unpickled
+    h = torch.zeros(3, 32)
+    assert model.normalized(0, h) is h
+
+
+def test_sides_past_32_bits_are_refused():
+    with pytest.raises(ValueError, match="16384"):
+        optim._workspace([1 << 31, 1], "cpu")
