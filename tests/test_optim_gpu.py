@@ -374,6 +374,21 @@ def test_many_matrices_and_two_graphs_that_share_a_pool(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(outs[k], want[2 * k:2 * k + 2]))
 
 
+@pytest.mark.parametrize("count", [13, 30, 64, 75])
+def test_large_matrices_that_share_the_device(count, cuda_device):
+    """Lists of equal and of different sizes, more than one launch takes among
+    them: each result is that of a call of its own, bit for bit."""
+    g = torch.Generator(device="cuda").manual_seed(18)
+    sizes = [(256, 513), (256, 256), (513, 256), (129, 130), (1, 1200), (300, 700), (256, 512), (140, 1000), (520, 560)]
+    mats = [_gradient(*sizes[(k * k) % len(sizes)], g) for k in range(count)]
+    once = [orthogonalize(t) for t in mats]
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(orthogonalize(mats), once))
+    equal = [_gradient(256, 513, g) for _ in range(count)]
+    got = orthogonalize(equal)
+    assert all(torch.equal(got[k], orthogonalize(equal[k])) for k in range(0, count, 5))
+
+
 def test_more_small_matrices_than_a_batch_holds(cuda_device):
     g = torch.Generator(device="cuda").manual_seed(17)
     mats = [_gradient(9 + k % 5, 20, g) for k in range(333)] + [_gradient(140, 150, g)]
