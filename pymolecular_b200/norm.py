@@ -9,6 +9,8 @@ between its layers when built with ``node_norm=True``.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import nn
 
@@ -17,16 +19,24 @@ from . import _native as nat
 DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_size(rows, cols, device):
+    return nat.lib().egnn_layer_norm_workspace_size(rows, cols)
+
+
 def _forward(x, weight, bias, eps, stats):
     """y and, where asked for, the (rows, 2) mean and 1 / sqrt(var + eps)."""
     rows, cols = x.shape
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     kept = x.new_empty((rows, 2), dtype=torch.float32) if stats else None
     p = weight if weight is not None else bias
+    lib = nat.lib()
     with nat.device_of(x):
-        nat.check(nat.lib().egnn_layer_norm_fwd(rows, cols, x.data_ptr(), x.stride(0), DTYPES[x.dtype], nat.ptr(weight),
-                                                nat.ptr(bias), nat.DTYPE_F32 if p is None else DTYPES[p.dtype], eps,
-                                                y.data_ptr(), nat.ptr(kept), nat.stream_ptr()), "egnn_layer_norm_fwd")
+        nat.check(lib.egnn_layer_norm_fwd(rows, cols, x.data_ptr(), x.stride(0), DTYPES[x.dtype],
+                                          None if weight is None else weight.data_ptr(),
+                                          None if bias is None else bias.data_ptr(),
+                                          nat.DTYPE_F32 if p is None else DTYPES[p.dtype], eps, y.data_ptr(),
+                                          kept.data_ptr() if stats else None, nat.stream_ptr()), "egnn_layer_norm_fwd")
     return y, kept
 
 
@@ -42,7 +52,7 @@ def _backward(ctx, dy):
     lib, ws, nbytes = nat.lib(), None, 0
     with nat.device_of(x):
         if need_w or need_b:
-            nbytes = lib.egnn_layer_norm_workspace_size(rows, cols)
+            nbytes = _workspace_size(rows, cols, x.get_device())
             ws = x.new_empty(nbytes, dtype=torch.uint8)
         nat.check(lib.egnn_layer_norm_bwd(rows, cols, x.data_ptr(), x.stride(0), dy.data_ptr(), dy.stride(0),
                                           DTYPES[x.dtype], nat.ptr(weight), DTYPES[pdt], stats.data_ptr(), nat.ptr(dx),
@@ -81,7 +91,8 @@ def layer_norm(x: torch.Tensor, layer: nn.LayerNorm) -> torch.Tensor:
     are float32 or of x's type, both of one type.  The result has x's type;
     statistics and sums are float32.
     """
-    if not x.is_cuda:
+    device = x.get_device()
+    if device < 0:
         raise ValueError("layer_norm takes CUDA tensors (pymolecular_b200 has no CPU path)")
     dtype, size, shape = x.dtype, x.shape, layer.normalized_shape
     if dtype not in DTYPES:
@@ -89,14 +100,17 @@ def layer_norm(x: torch.Tensor, layer: nn.LayerNorm) -> torch.Tensor:
     if len(shape) != 1 or not size or size[-1] != shape[0]:
         raise ValueError(f"x must be (..., C) for a LayerNorm over its last axis alone, got {tuple(size)} and "
                          f"normalized_shape {tuple(shape)}")
-    weight, bias = layer.weight, layer.bias
+    params = layer._parameters   # spares nn.Module's lookup; a parametrised layer has none there
+    weight = params["weight"] if "weight" in params else layer.weight
+    bias = params["bias"] if "bias" in params else layer.bias
     needs_grad = x.requires_grad
     for p in (weight, bias):
         if p is None:
             continue
-        if p.device != x.device:
+        if p.get_device() != device:
             raise ValueError(f"the layer's parameters must be on {x.device}, got {p.device}")
-        if p.dtype not in (torch.float32, dtype) or (weight is not None and p.dtype != weight.dtype):
+        code = p.dtype
+        if code is not torch.float32 and code is not dtype or weight is not None and code is not weight.dtype:
             raise TypeError(f"the layer's parameters must be float32 or {dtype}, both of one type, got {p.dtype}")
         needs_grad = needs_grad or p.requires_grad
     rows = x if len(size) == 2 else x.reshape(-1, shape[0])
