@@ -101,6 +101,18 @@ def test_against_float64(cols, dtype, cuda_device):
         assert torch.equal(layer_norm(x, layer), got["y"])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [321, 383, 385, 511])
+def test_widths_of_scalar_rows(cols, dtype, cuda_device):
+    """12 and 16 scalars to a lane."""
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x, layer = _features(777, cols, g, dtype, pad=3), _layer(cols, g)
+    dy = torch.randn(777, cols, device="cuda", generator=g).to(dtype)
+    got, want = _run(x, layer, dy), _oracle(x, layer, dy)
+    for k in got:
+        _check(k, got[k], want[k])
+
+
 @pytest.mark.parametrize("rows,cols", [(1, 64), (2, 128), (1850, 64), (9939, 128), (4001, 256), (70000, 40)])
 def test_row_counts(rows, cols, cuda_device):
     g = torch.Generator(device="cuda").manual_seed(rows)
