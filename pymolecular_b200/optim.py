@@ -98,9 +98,11 @@ def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = S
     fields, out = [0] * (6 * len(mats)), [None] * len(mats)
     for (size, code), members in groups.items():
         rows, cols = size
-        made = torch.empty((len(members), rows, cols), dtype=mats[members[0]].dtype, device=device)
+        n = len(members)
+        made = mats[members[0]].new_empty((n * rows, cols))
         at, step, both = made.data_ptr(), rows * cols * made.element_size(), rows | cols << 32
-        for k, o in zip(members, made.unbind(0)):
+        # unsafe: `made` itself is not used beside its parts (which then are no views for autograd, and quicker)
+        for k, o in zip(members, made.unsafe_split_with_sizes([rows] * n) if n > 1 else (made,)):
             out[k] = o
             fields[6 * k:6 * k + 6] = ptrs[k], at, strides[k], cols, both, code
             at += step
@@ -127,7 +129,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
         raise ValueError("muon_step takes one gradient and one momentum buffer for each parameter")
     if not params:
         return
-    if len({id(t) for t in (*params, *buffers)}) < 2 * len(params):
+    if len(set(map(id, params + buffers))) < 2 * len(params):
         raise ValueError("a parameter or momentum buffer is given twice")
     device = params[0].get_device()
     if device < 0:
