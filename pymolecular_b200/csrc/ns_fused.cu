@@ -16,11 +16,10 @@
 // and 13 for m > 32, tensor memory n to 1024.
 //
 // What bounds it: a chain of three dependent products a step, on one SM.  A step of
-// 128 x 257 takes 15,000 cycles, its products alone 8,300 (three half-precision
+// 128 x 257 takes 14,000 cycles, its products alone 8,300 (three half-precision
 // products each), the rest are accumulators on their way through the registers.
-// 5 steps of one 64 x 129 take 31 us, of one 128 x 257 and of 35 of them 55 us, against
-// 71, 93 and 130 us in the kernel for large matrices; from 128 x 321 on that one takes
-// 97 us.  A matrix on a cluster of two blocks was slower (65 us for the 35): 64 KB
+// 5 steps of one 64 x 129 take 30 us, of one 128 x 257 and of 35 of them 53 us, against
+// 71, 93 and 130 us in the kernel for large matrices, which takes 100 us for 128 x 321.  A matrix on a cluster of two blocks was slower (65 us for the 35, then 55 without): 64 KB
 // through distributed shared memory cost 9,000 cycles a step.
 #include <atomic>
 
@@ -368,35 +367,49 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
     bool ok = true;
 #pragma unroll 1
     for (int step = 0; step < q.steps && ok; ++step) {
-      float v[32], w[32];
+      // What does not wait for a product is fetched before the wait.  An accumulator is read
+      // to its end before the first half is handed over, where the products of that half
+      // write to its place.
+      float v[32];   // A, then B, then X
+      auto read_a = [&](int h) {
+        float t[16], x[16];
+        const uint32_t c = lanes + piece * 32 + 16 * h;
+        tmem_ld16x2(tA + c, tAx + c, t, x);
+        for (int j = 1; j < sums; ++j) {
+          float u[16];
+          tmem_ld16(tmem + j * kSlotCols + c, u);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) t[k] += u[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[16 * h + k] = (fmaf(t[k], loss_n, t[k]) + x[k]) * fA;
+      };
       if (!(ok = wait_bar(&bar.a_done, step, gave_up, q.wait_polls))) break;
       if (a_here) {
-        tmem_ld32(tA + lanes + piece * 32, v);
-        for (int j = 1; j < sums; ++j) {
-          tmem_ld32(tmem + j * kSlotCols + lanes + piece * 32, w);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] += w[k];
-        }
-        tmem_ld32(tAx + lanes + piece * 32, w);
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = fmaf(v[k], loss_n, v[k]) + w[k];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] *= fA;
+        read_a(0);
+        if (sums > 1) read_a(1);   // A A goes where the sums are
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (a_here) store_pairs16(ah, ah + at, h, v + 16 * h);
+        if (a_here) {
+          if (h == 1 && sums == 1) read_a(1);
+          store_pairs16(ah, ah + at, h, v + 16 * h);
+        }
         arrive(&bar.a_ready[h]);
       }
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] *= fbA;
       if (!(ok = wait_bar(&bar.aa_done, step, gave_up))) break;
       if (a_here) {
-        load_pairs32(ah, ah + at, w);   // this thread's own
-        tmem_ld32(tAA + lanes + piece * 32, v);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) w[k] = fmaf(fbA, w[k], fcAA * fmaf(v[k], loss_m, v[k]));
-        tmem_ld32(tAAx + lanes + piece * 32, v);
+        for (int h = 0; h < 2; ++h) {
+          float t[16], x[16];
+          const uint32_t c = lanes + piece * 32 + 16 * h;
+          tmem_ld16x2(tAA + c, tAAx + c, t, x);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = fmaf(fcAA, v[k], w[k]);
+          for (int k = 0; k < 16; ++k)
+            v[16 * h + k] = fmaf(fcAA, x[k], fmaf(fcAA, fmaf(t[k], loss_m, t[k]), v[16 * h + k]));
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -412,15 +425,24 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
 #pragma unroll 1
       for (int k = 0; k < chunks; ++k) {
         const int slot = k % kSlots;
-        if (!(ok = wait_bar(&bar.slot_done[slot], slot_use(step, k), gave_up))) break;
         const int c0 = k * kSlotCols + piece * 32;
         const bool here = rows_here && c0 < n16;
         const uint32_t hi = xh + k * (2 * R * 128), lo = hi + xt;
-        if (here) {
-          tmem_ld32(tmem + lanes + slot * kSlotCols + piece * 32, v);
-          load_pairs32(hi, lo, w);
+        if (here) {   // this thread's own
+          load_pairs32(hi, lo, v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(q.a, w[j], fX * fmaf(v[j], loss_m, v[j]));
+          for (int j = 0; j < 32; ++j) v[j] *= q.a;
+        }
+        if (!(ok = wait_bar(&bar.slot_done[slot], slot_use(step, k), gave_up))) break;
+        if (here) {
+          float t[16], u[16];
+          const uint32_t c = tmem + lanes + slot * kSlotCols + piece * 32;
+          tmem_ld16x2(c, c + 16, t, u);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            v[j] = fmaf(fX, fmaf(t[j], loss_m, t[j]), v[j]);
+            v[16 + j] = fmaf(fX, fmaf(u[j], loss_m, u[j]), v[16 + j]);
+          }
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
