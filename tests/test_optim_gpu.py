@@ -374,6 +374,22 @@ def test_many_matrices_and_two_graphs_that_share_a_pool(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(outs[k], want[2 * k:2 * k + 2]))
 
 
+@pytest.mark.parametrize("shapes", [[(64, 2000)], [(257, 2100), (40, 50)], [(256, 513)] * 30])
+def test_waits_that_run_out_in_pieces_and_wide_tiles(shapes, cuda_device, monkeypatch):
+    """As above, for long sums in pieces, a side stream, and tiles of 128 columns."""
+    lib = nat.lib()
+    g = torch.Generator(device="cuda").manual_seed(19)
+    mats = [_gradient(*s, g) for s in shapes]
+    monkeypatch.delenv("EGNN_DEBUG_WAIT_POLLS", raising=False)
+    want = orthogonalize(mats)
+    assert lib.egnn_device_status(nat.stream_ptr()) == nat.EGNN_OK, nat.last_error()
+    monkeypatch.setenv("EGNN_DEBUG_WAIT_POLLS", "0")
+    orthogonalize(mats)
+    assert lib.egnn_device_status(nat.stream_ptr()) == nat.EGNN_ERR_CUDA and "timed out" in nat.last_error()
+    monkeypatch.delenv("EGNN_DEBUG_WAIT_POLLS")
+    assert all(torch.equal(a, b) for a, b in zip(orthogonalize(mats), want))
+
+
 @pytest.mark.parametrize("count", [13, 30, 64, 75])
 def test_large_matrices_that_share_the_device(count, cuda_device):
     """Lists of equal and of different sizes, more than one launch takes among
