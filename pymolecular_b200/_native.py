@@ -208,19 +208,35 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_device = _raw_stream = None   # torch's functions for the current device and its stream's handle
+
+
+def _bind():
+    global _device, _raw_stream
+    import torch
+    torch.cuda.current_device()   # initialises CUDA, which the functions below do not
+    # a tenth of the cost of making a Stream object
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def stream_ptr(stream=None) -> int:
     """Handle of `stream`, or of the current stream of the current device."""
-    import torch
     if stream is not None:
         return stream.cuda_stream
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # a tenth of the cost of making a Stream object
-    return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
+    if _device is None:
+        _bind()
+    return _raw_stream(_device())
 
 
 def device_of(t):
     """Context in which `t`'s device is the current one."""
+    if _device is None:
+        _bind()
+    if t.get_device() == _device():
+        return _SAME
     import torch
-    return _SAME if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return torch.cuda.device(t.device)
 
 
 _SAME = contextlib.nullcontext()
