@@ -82,10 +82,23 @@ bool size_built(int rows, int cols) {
 
 bool is_large(int rows, int cols) { return !ns_fused_fits(std::min(rows, cols), std::max(rows, cols)); }
 
-// Workspace of a matrix that a block's shared memory does not hold.
-void carve(Carver& c, int rows, int cols) {
-  if (rows && cols && is_large(rows, cols)) ns_grid_carve(c, rows, cols);
-}
+// Workspace of the matrices that a block's shared memory does not hold: that of the
+// batch of them which needs most, since batches run one after another.
+struct Need {
+  Carver c{nullptr};
+  size_t most;
+  int64_t large = 0;
+  Need() {
+    c.take<float>(1);
+    most = c.size();
+  }
+  void add(int rows, int cols) {
+    if (!rows || !cols || !is_large(rows, cols)) return;
+    if (large++ % kNsLarge == 0) c.off = 0;
+    ns_grid_carve(c, rows, cols);
+    most = std::max(most, c.size());
+  }
+};
 
 // The matrices that fit a block's shared memory in batches of one launch, the
 // large ones in batches of their own.  Everything is checked before the first
@@ -94,20 +107,18 @@ template <class Fill>
 int run_all(const char* what, int64_t count, const Fill& fill, const NsScalars& q, void* ws, size_t ws_bytes,
             cudaStream_t s) {
   if (count == 0) return EGNN_OK;
-  Carver need(nullptr);
-  need.take<float>(1);
+  Need need;
   NsItem it;
-  int64_t small_count = 0, large_count = 0;
+  int64_t small_count = 0;
   for (int64_t i = 0; i < count; ++i) {
     EGNN_TRY(fill(i, it));
-    carve(need, it.rows, it.cols);
-    if (it.rows && it.cols) ++(is_large(it.rows, it.cols) ? large_count : small_count);
+    need.add(it.rows, it.cols);
+    small_count += it.rows && it.cols && !is_large(it.rows, it.cols);
   }
-  if (!ws || ws_bytes < need.size()) return fail(EGNN_ERR_WORKSPACE, "%s: workspace too small", what);
+  if (!ws || ws_bytes < need.most) return fail(EGNN_ERR_WORKSPACE, "%s: workspace too small", what);
   if (reinterpret_cast<uintptr_t>(ws) & 255u)
     return fail(EGNN_ERR_INVALID_ARG, "%s: the workspace must start on a 256-byte boundary", what);
-  Carver c(ws);
-  c.take<float>(1);
+  const Carver c(ws);
   // A few small matrices among large ones (embeddings among wide layers) run beside
   // them, on SMs that the large ones leave: five of up to 128 x 31 with 200 x 333,
   // 64 x 1100 and 513 x 97 take 171 us, one kernel after the other 191.
@@ -124,7 +135,7 @@ int run_all(const char* what, int64_t count, const Fill& fill, const NsScalars& 
       return was ? join_side(main_s) : EGNN_OK;
     }
     ~Side() { join(); }   // also on an early return, so that no capture is left forked
-  } side(s, large_count > 0 && small_count > 0 && small_count <= num_sms_current() / 8);
+  } side(s, need.large > 0 && small_count > 0 && small_count <= num_sms_current() / 8);
   EGNN_TRY(side.status);
   const int spare = side.on ? (int)small_count : 0;
   NsBatch small, large;
@@ -134,7 +145,7 @@ int run_all(const char* what, int64_t count, const Fill& fill, const NsScalars& 
     if (it.rows == 0 || it.cols == 0) continue;
     NsBatch& b = is_large(it.rows, it.cols) ? large : small;
     b.it[b.count] = it;
-    if (++b.count == kNsItems) {
+    if (++b.count == (&b == &large ? kNsLarge : kNsItems)) {
       EGNN_TRY(&b == &large ? ns_grid(b, c, q, spare, s) : ns_fused(b, q, side.stream));
       b.count = 0;
     }
@@ -151,13 +162,12 @@ using namespace egnn;
 
 extern "C" size_t egnn_orthogonalize_workspace_size(int64_t count, const int32_t* sizes) {
   if (count < 0 || (count > 0 && !sizes)) return 0;
-  Carver c(nullptr);
-  c.take<float>(1);
+  Need need;
   for (int64_t i = 0; i < count; ++i) {
     if (!size_built(sizes[2 * i], sizes[2 * i + 1])) return 0;
-    carve(c, sizes[2 * i], sizes[2 * i + 1]);
+    need.add(sizes[2 * i], sizes[2 * i + 1]);
   }
-  return c.size();
+  return need.most;
 }
 
 extern "C" int egnn_orthogonalize(int64_t count, const egnn_matrix* m, const egnn_ns_options* o, void* ws,

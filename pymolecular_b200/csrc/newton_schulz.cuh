@@ -14,6 +14,7 @@ namespace egnn {
 // Matrices of one batch: as many as fill the device with one block each (10 KB of kernel
 // parameters; 140 of 128 x 257 take 60 us, in batches of 64 166 us).
 constexpr int kNsItems = 160;
+constexpr int kNsLarge = 64;   // matrices of a batch that go through the workspace, which batches share
 constexpr int kNsMaxSteps = 64;
 
 struct NsItem {
@@ -84,7 +85,7 @@ bool ns_fused_fits(int m, int n);
 int ns_fused(const NsBatch& b, const NsScalars& q, cudaStream_t s);
 // The matrices of the batch on the whole device but `spare` SMs, with workspace
 // from `c`; ns_grid_carve takes what one matrix needs.
-int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, int spare, cudaStream_t s);
+int ns_grid(const NsBatch& b, Carver c, const NsScalars& q, int spare, cudaStream_t s);
 void ns_grid_carve(Carver& c, int rows, int cols);
 // Waits that ran out since the last call.
 int ns_fused_take_timeouts();

@@ -58,7 +58,7 @@ struct Work {
   float* part;           // pieces of A
   double* partial;       // sums of squares of the parts of U
 };
-constexpr int kItems = 64;   // matrices of one launch
+constexpr int kItems = kNsLarge;   // matrices of one launch
 struct Grid {
   NsItem it[kItems];
   Work w[kItems];
@@ -804,7 +804,7 @@ void ns_grid_carve(Carver& c, int rows, int cols) {
   carve_work(c, Shape(it));
 }
 
-int ns_grid(const NsBatch& b, Carver& c, const NsScalars& q, int spare, cudaStream_t s) {
+int ns_grid(const NsBatch& b, Carver c, const NsScalars& q, int spare, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
   const uint64_t bit = device_bit();
   if (!(ready.load() & bit)) {

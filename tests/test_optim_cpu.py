@@ -169,3 +169,13 @@ def test_models_from_before_there_were_norms():
 def test_sides_past_32_bits_are_refused():
     with pytest.raises(ValueError, match="16384"):
         optim._workspace([1 << 31, 1], "cpu")
+
+
+def test_workspace_is_that_of_the_largest_batch():
+    def size(*sizes):
+        flat = [v for s in sizes for v in s]
+        return nat.lib().egnn_orthogonalize_workspace_size(len(sizes), (C.c_int32 * len(flat))(*flat))
+
+    full = size(*[(200, 333)] * 64)
+    assert size(*[(200, 333)] * 63) < full == size(*[(200, 333)] * 65) == size(*[(200, 333)] * 1000)
+    assert size(*[(200, 333)] * 64, *[(64, 64)] * 99, *[(400, 1333)] * 64, (1, 1)) == size(*[(400, 1333)] * 64)

@@ -405,6 +405,16 @@ def test_large_matrices_that_share_the_device(count, cuda_device):
     assert all(torch.equal(got[k], orthogonalize(equal[k])) for k in range(0, count, 5))
 
 
+def test_batches_share_the_workspace(cuda_device):
+    """More large matrices than a batch holds, small ones between them."""
+    g = torch.Generator(device="cuda").manual_seed(20)
+    sizes = [(130, 140), (64, 64), (300, 200), (20, 2000)]
+    mats = [_gradient(*sizes[k % 4], g) for k in range(300)]
+    got = orthogonalize(mats)
+    for k in (0, 1, 84, 85, 86, 87, 170, 171, 172, 256, 258, 298, 299):
+        assert torch.equal(got[k], orthogonalize(mats[k]))
+
+
 def test_more_small_matrices_than_a_batch_holds(cuda_device):
     g = torch.Generator(device="cuda").manual_seed(17)
     mats = [_gradient(9 + k % 5, 20, g) for k in range(333)] + [_gradient(140, 150, g)]
