@@ -512,6 +512,16 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const float loss = ns_mean_loss(4 * segment);
     int seg = 0, outs = 0, sent = 0;
+    // The readers' arrival at `written`.  A warp arrives again only when the last round is
+    // complete: arrivals are counted, not the warps, and a fast one's second would stand for a slow
+    // one's first.
+    auto arrive_written = [&]() {
+      __syncwarp();
+      if (outs && !(ok = wait_bar(&bar.written, outs - 1, gave_up))) return false;
+      if (lane == 0) mbar_arrive(&bar.written);
+      ++outs;
+      return true;
+    };
     uint32_t parity = 0;   // of each stage's next filling
 #pragma unroll 1
     for (int p = 0, phase_of_step = 0, cur = 0; p < phases && ok; ++p, ++phase_of_step) {
@@ -601,10 +611,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
         const bool ring_free = t + group >= f.tiles;
         auto hand_on = [&]() {   // true in warp 2 when all have written
           fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.written);
-          if (warp == 2) ok = wait_bar(&bar.written, outs, gave_up);
-          ++outs;
+          if (!arrive_written()) return false;
+          if (warp == 2) ok = wait_bar(&bar.written, outs - 1, gave_up);
           return warp == 2 && ok;
         };
         auto out_free = [&]() {   // the copies out of the blocks behind the ring have read them
@@ -630,9 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
             if (tile == 64) {
               if (!out_free()) return;
             } else if (mode != 0) {   // every reader has taken its part of the old tile out of the ring
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bar.written);
-              if (!(ok = wait_bar(&bar.written, outs++, gave_up))) return;
+              if (!arrive_written() || !(ok = wait_bar(&bar.written, outs - 1, gave_up))) return;
             }
             char* const from = tile == 64 ? out : ring;
             if (here) {
@@ -679,10 +685,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
       }
       if (!ok) break;
       if (apart || mode == 3) {   // what all readers have stored
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.written);
-        if (warp == 2 && !(ok = wait_bar(&bar.written, outs, gave_up))) break;
-        ++outs;
+        if (!arrive_written()) break;
+        if (warp == 2 && !(ok = wait_bar(&bar.written, outs - 1, gave_up))) break;
       }
       if (warp == 2 && lane == 0) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

@@ -415,6 +415,19 @@ def test_batches_share_the_workspace(cuda_device):
         assert torch.equal(got[k], orthogonalize(mats[k]))
 
 
+@pytest.mark.parametrize("shapes", [[(100, 2192)], [(100, 2192), (64, 1100)], [(1, 16384), (257, 2100)],
+                                    [(256, 513)] * 30, [(300, 700)] * 20])
+def test_many_calls_give_the_same(shapes, cuda_device):
+    """Blocks with no tile of a product, one, and several: what warps hand over
+    must be complete however far they are apart."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    mats = [_gradient(*s, g) for s in shapes]
+    want = [orthogonalize(t) for t in mats]
+    for _ in range(60):
+        outs = [orthogonalize(mats) for _ in range(10)]
+        assert all(torch.equal(a, b) for out in outs for a, b in zip(out, want))
+
+
 def test_more_small_matrices_than_a_batch_holds(cuda_device):
     g = torch.Generator(device="cuda").manual_seed(17)
     mats = [_gradient(9 + k % 5, 20, g) for k in range(333)] + [_gradient(140, 150, g)]
