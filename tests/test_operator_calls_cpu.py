@@ -1,0 +1,20 @@
+"""Calls of the layer norm, the orthogonalisation and the momentum step that
+have to be refused, or answered without a launch, shown without a GPU."""
+import pytest
+import torch
+from torch import nn
+
+from pymolecular_b200 import layer_norm
+
+
+@pytest.mark.parametrize("name", ["weight", "bias"])
+@pytest.mark.parametrize("shape", [(7,), (9,), (1,), (0,), (8, 1), (1, 8), ()])
+def test_parameters_of_another_shape_are_refused(name, shape):
+    """A kernel reads C elements of the weight and bias and writes C of their
+    gradients, however many there are."""
+    layer = nn.LayerNorm(8)
+    setattr(layer, name, nn.Parameter(torch.ones(shape)))
+    with pytest.raises(ValueError, match="normalized_shape"):
+        layer_norm(torch.zeros(4, 8), layer)
+    with pytest.raises(RuntimeError):   # as nn.LayerNorm does
+        layer(torch.zeros(4, 8))
