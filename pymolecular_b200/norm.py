@@ -91,25 +91,24 @@ def layer_norm(x: torch.Tensor, layer: nn.LayerNorm) -> torch.Tensor:
     are float32 or of x's type, both of one type.  The result has x's type;
     statistics and sums are float32.
     """
-    params = layer._parameters   # spares nn.Module's lookup; a parametrised layer has none there
-    weight = params["weight"] if "weight" in params else layer.weight
-    bias = params["bias"] if "bias" in params else layer.bias
-    dtype, size, shape = x.dtype, x.shape, tuple(layer.normalized_shape)
-    for p in (weight, bias):   # the kernels read C elements of each, and write as many of their gradients
-        if p is not None and p.shape != shape:
-            raise ValueError(f"the layer's parameters must be of its normalized_shape {shape}, got {tuple(p.shape)}")
     device = x.get_device()
     if device < 0:
         raise ValueError("layer_norm takes CUDA tensors (pymolecular_b200 has no CPU path)")
+    dtype, size, shape = x.dtype, x.shape, tuple(layer.normalized_shape)
     if dtype not in DTYPES:
         raise TypeError(f"x must be float32, bfloat16 or float16, got {dtype}")
     if len(shape) != 1 or not size or size[-1] != shape[0]:
         raise ValueError(f"x must be (..., C) for a LayerNorm over its last axis alone, got {tuple(size)} and "
                          f"normalized_shape {shape}")
+    params = layer._parameters   # spares nn.Module's lookup; a parametrised layer has none there
+    weight = params["weight"] if "weight" in params else layer.weight
+    bias = params["bias"] if "bias" in params else layer.bias
     needs_grad = x.requires_grad
     for p in (weight, bias):
         if p is None:
             continue
+        if p.shape != shape:   # the kernels read C elements of each, and write as many of their gradients
+            raise ValueError(f"the layer's parameters must be of its normalized_shape {shape}, got {tuple(p.shape)}")
         if p.get_device() != device:
             raise ValueError(f"the layer's parameters must be on {x.device}, got {p.device}")
         code = p.dtype

@@ -7,6 +7,13 @@ from torch import nn
 from pymolecular_b200 import layer_norm
 
 
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on device 0."""
+
+    def get_device(self):
+        return 0
+
+
 @pytest.mark.parametrize("name", ["weight", "bias"])
 @pytest.mark.parametrize("shape", [(7,), (9,), (1,), (0,), (8, 1), (1, 8), ()])
 def test_parameters_of_another_shape_are_refused(name, shape):
@@ -15,6 +22,6 @@ def test_parameters_of_another_shape_are_refused(name, shape):
     layer = nn.LayerNorm(8)
     setattr(layer, name, nn.Parameter(torch.ones(shape)))
     with pytest.raises(ValueError, match="normalized_shape"):
-        layer_norm(torch.zeros(4, 8), layer)
+        layer_norm(torch.zeros(4, 8).as_subclass(OnDevice), layer)
     with pytest.raises(RuntimeError):   # as nn.LayerNorm does
         layer(torch.zeros(4, 8))
