@@ -20,7 +20,8 @@ def test_parameters_of_another_shape_are_refused(name, shape):
     """A kernel reads C elements of the weight and bias and writes C of their
     gradients, however many there are."""
     layer = nn.LayerNorm(8)
-    setattr(layer, name, nn.Parameter(torch.ones(shape)))
+    for n in ("weight", "bias"):
+        setattr(layer, n, nn.Parameter(torch.ones(shape if n == name else 8).as_subclass(OnDevice)))
     with pytest.raises(ValueError, match="normalized_shape"):
         layer_norm(torch.zeros(4, 8).as_subclass(OnDevice), layer)
     with pytest.raises(RuntimeError):   # as nn.LayerNorm does
