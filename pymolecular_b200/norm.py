@@ -13,6 +13,7 @@ import functools
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -122,7 +123,9 @@ def layer_norm(x: torch.Tensor, layer: nn.LayerNorm) -> torch.Tensor:
         weight = weight.contiguous()
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    if needs_grad and torch.is_grad_enabled():
+    # Through autograd also what has to be recorded, or refused, without a gradient: dual tensors
+    # of forward mode (the Function has no jvp), and tracing, which makes tensors of sizes.
+    if needs_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 or type(size[-1]) is not int:
         y = _LayerNormFn.apply(rows, weight, bias, layer.eps)
     else:
         y = _forward(rows, weight, bias, layer.eps, False)[0]
