@@ -61,7 +61,8 @@ def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = S
     if isinstance(g, torch.Tensor):
         if g.dim() < 2:
             raise ValueError("orthogonalize takes matrices")
-        mats = g.detach().reshape(-1, *g.shape[-2:]).unbind(0)
+        batch = g.detach()
+        mats = batch.flatten(0, -3).unbind(0) if g.dim() > 2 else (batch,)   # reshape(-1, ...) refuses empty sides
         if not mats:
             return torch.empty_like(g, memory_format=torch.contiguous_format)
     else:

@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch import nn
 
-from pymolecular_b200 import layer_norm
+from pymolecular_b200 import layer_norm, orthogonalize
 
 
 class OnDevice(torch.Tensor):
@@ -26,3 +26,9 @@ def test_parameters_of_another_shape_are_refused(name, shape):
         layer_norm(torch.zeros(4, 8).as_subclass(OnDevice), layer)
     with pytest.raises(RuntimeError):   # as nn.LayerNorm does
         layer(torch.zeros(4, 8))
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0, 0), (3, 0, 4), (2, 3, 4, 0)])
+def test_matrices_with_an_empty_side_come_as_far_as_others(shape):
+    with pytest.raises(ValueError, match="CUDA"):
+        orthogonalize(torch.zeros(shape))

@@ -5,7 +5,7 @@ import torch
 from torch import nn
 from torch.autograd import forward_ad
 
-from pymolecular_b200 import layer_norm
+from pymolecular_b200 import layer_norm, orthogonalize
 
 pytestmark = pytest.mark.gpu
 
@@ -40,3 +40,11 @@ def test_traced_call_computes(shape, cuda_device):
         with torch.set_grad_enabled(grad):
             traced = torch.jit.trace(lambda t: 2 * layer_norm(t, layer), (x,))
             assert torch.equal(traced(other), 2 * layer_norm(other, layer))
+
+
+@pytest.mark.parametrize("shape", [(0, 5), (5, 0), (0, 0), (3, 0, 4), (0, 3, 4), (2, 3, 4, 0), (2, 0, 3, 4)])
+def test_matrices_with_an_empty_side(shape, cuda_device):
+    """Alone and in batches, as in lists."""
+    for dtype in (torch.float32, torch.bfloat16):
+        out = orthogonalize(torch.zeros(shape, dtype=dtype, device=cuda_device))
+        assert out.shape == shape and out.dtype == dtype and out.device == cuda_device
