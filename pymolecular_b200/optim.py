@@ -48,6 +48,11 @@ def _workspace(sizes: Sequence[int], device) -> Tuple[torch.Tensor, int]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
+def _refuse_tracing(t: torch.Tensor) -> None:
+    if t.dim() and type(t.shape[0]) is not int:   # torch.jit.trace makes tensors of sizes
+        raise RuntimeError("torch.jit.trace does not see what these kernels write: their results are written by pointer")
+
+
 def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = STEPS,
                   coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = EPS):
     """The matrix, batch of matrices (..., m, n) or list of matrices `g` with
@@ -72,6 +77,7 @@ def orthogonalize(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = S
     device = mats[0].get_device()
     if device < 0:
         raise ValueError("orthogonalize takes CUDA tensors (pymolecular_b200 has no CPU path)")
+    _refuse_tracing(mats[0])
     groups, sizes, ptrs, strides, copies = {}, [], [], [], []
     for k, t in enumerate(mats):
         size, code = t.shape, DTYPES.get(t.dtype)
@@ -135,6 +141,7 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
     device = params[0].get_device()
     if device < 0:
         raise ValueError("muon_step takes CUDA tensors (pymolecular_b200 has no CPU path)")
+    _refuse_tracing(params[0])
     on_device = isinstance(lr, torch.Tensor)
     if on_device and (lr.numel() != 1 or lr.dtype != torch.float32 or lr.get_device() != device):
         raise ValueError("lr must be a number or one float32 on the parameters' device")

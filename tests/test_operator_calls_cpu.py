@@ -4,7 +4,7 @@ import pytest
 import torch
 from torch import nn
 
-from pymolecular_b200 import layer_norm, orthogonalize
+from pymolecular_b200 import layer_norm, muon_step, orthogonalize
 
 
 class OnDevice(torch.Tensor):
@@ -32,3 +32,13 @@ def test_parameters_of_another_shape_are_refused(name, shape):
 def test_matrices_with_an_empty_side_come_as_far_as_others(shape):
     with pytest.raises(ValueError, match="CUDA"):
         orthogonalize(torch.zeros(shape))
+
+
+def test_tracing_of_results_written_by_pointer_is_refused():
+    def step(w):
+        muon_step([w], [w.clone().as_subclass(OnDevice)], [w.clone().as_subclass(OnDevice)], lr=0.1)
+        return w
+
+    for call in (orthogonalize, lambda w: orthogonalize([w, w])[0], step):
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(lambda t: call(t.as_subclass(OnDevice)), (torch.ones(4, 4),))
