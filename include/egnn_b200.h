@@ -344,8 +344,9 @@ EGNN_API int egnn_layer_norm_bwd(int64_t rows, int32_t cols, const void* x, int6
 /* The iteration: X0 = G / (|G|_F + eps), transposed where rows > cols, then
  * `steps` times X <- a X + (b A + c A A) X with A = X X^T.  It acts on the
  * singular values alone: s <- a s + b s^3 + c s^5.  The coefficients must
- * keep the singular values that start in [0, 1] below 1024 in every step
- * (EGNN_ERR_INVALID_ARG otherwise). */
+ * keep the singular values that start in [0, 1] below 1024 in every step,
+ * and before the last step below 16 |a|^k after k steps, so that small ones
+ * keep their bits beside the largest (EGNN_ERR_INVALID_ARG otherwise). */
 typedef struct {
   int32_t steps;     /* 0 .. 64 */
   int32_t reserved;  /* 0 */
@@ -370,8 +371,10 @@ typedef struct {
 EGNN_API size_t egnn_orthogonalize_workspace_size(int64_t count, const int32_t* sizes);
 
 /* out_k = the orthogonalised in_k for every matrix of the HOST array `m`
- * (read before the call returns).  Products are as exact as float32's.
- * Deterministic.  No counterpart in the reference. */
+ * (read before the call returns).  The products' operands have 22 bits,
+ * their sums float32's 24: against float64 the result of the usual steps is
+ * 0.6 to 1.6 times as far off as the same iteration in float32 (128 x 257: 0.9,
+ * 16 x 16384: 1.6).  Deterministic.  No counterpart in the reference. */
 EGNN_API int egnn_orthogonalize(int64_t count, const egnn_matrix* m, const egnn_ns_options* o, void* workspace,
                                 size_t workspace_bytes, void* stream);
 

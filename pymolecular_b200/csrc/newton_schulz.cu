@@ -40,27 +40,46 @@ double odd_poly_max(const egnn_ns_options& o, double r) {
   return most;
 }
 
-// 2^e with size 2^e near 2^14: a factor 4 below fp16's largest value.
-float scale_for(double size) {
-  if (!(size > 0.0)) return 1.f;
-  const int e = 14 - (int)std::ceil(std::log2(size));
-  return (float)std::ldexp(1.0, std::max(-60, std::min(60, e)));
+// Largest |p(s) / s| of it on [0, r]: at the ends or where its derivative in s^2 is zero.
+double even_poly_max(const egnn_ns_options& o, double r) {
+  auto p = [&](double t) { return std::fabs(o.a + t * (o.b + t * o.c)); };
+  double most = std::max(p(0.0), p(r * r));
+  const double t = o.c != 0.0 ? -o.b / (2.0 * o.c) : -1.0;
+  if (t > 0.0 && t < r * r) most = std::max(most, p(t));
+  return most;
 }
 
-// Checks the options and derives the scales from how far the singular values can grow.
+// The least e with x <= 2^e, within what the kernels work with.
+int exponent_above(double x) {
+  if (!(x > 0.0)) return -kNsMostExp;
+  return (int)std::max<double>(-kNsMostExp, std::min<double>(kNsMostExp, std::ceil(std::log2(x))));
+}
+
+// Checks the options and derives the bounds of the scales from how far the singular values can grow.
 int scalars(const char* what, const egnn_ns_options& o, NsScalars& q) {
   if (o.steps < 0 || o.steps > kNsMaxSteps) return fail(EGNN_ERR_INVALID_ARG, "%s: steps must be 0 .. %d", what, kNsMaxSteps);
   if (!(o.eps >= 0.0) || !std::isfinite(o.eps)) return fail(EGNN_ERR_INVALID_ARG, "%s: eps must not be negative", what);
   if (!std::isfinite(o.a) || !std::isfinite(o.b) || !std::isfinite(o.c))
     return fail(EGNN_ERR_INVALID_ARG, "%s: coefficients must be finite", what);
-  double r = 1.0, most = 1.0;
+  q = NsScalars{};
+  // A scale follows the largest value that the bound allows, while small ones go with |a| in a
+  // step.  Entries near 2^-12 of the bound (1 / sqrt(m n) at the largest sides) keep their 22 bits
+  // down to another 2^-4; behind that the error grows past float32's
+  // (14 times at 2^-5: 1024 x 4096, coefficients 0.141, -4.726, 0.285).
+  double r = 1.0, small = 1.0;
   for (int k = 0; k < o.steps; ++k) {
+    q.growth[k] = (int8_t)exponent_above(even_poly_max(o, r));
     r = odd_poly_max(o, r);
     if (!(r < 1024.0))
       return fail(EGNN_ERR_INVALID_ARG, "%s: these coefficients let the singular values grow past 1024", what);
-    most = std::max(most, r);
+    q.bound[k + 1] = (int8_t)exponent_above(r);
+    small *= std::fabs(o.a);
+    if (k + 1 < o.steps && r > 16.0 * small)
+      return fail(EGNN_ERR_INVALID_ARG, "%s: these coefficients let small singular values fall too far behind the largest", what);
   }
-  q = NsScalars{};
+  q.a_exp = exponent_above(std::fabs(o.a));
+  q.b_exp = exponent_above(std::fabs(o.b));
+  q.c_exp = exponent_above(std::fabs(o.c));
   q.a = (float)o.a;
   q.b = (float)o.b;
   q.c = (float)o.c;
@@ -70,9 +89,6 @@ int scalars(const char* what, const egnn_ns_options& o, NsScalars& q) {
   const char* polls = std::getenv("EGNN_DEBUG_WAIT_POLLS");
   const long limit = polls && *polls ? std::strtol(polls, nullptr, 10) : -1;
   q.wait_polls = limit < 0 ? 1 << 22 : (int)std::min<long>(limit, 1L << 22);
-  q.sx = scale_for(most);
-  q.sa = scale_for(most * most);
-  q.sb = scale_for(std::fabs(o.b) * most * most + std::fabs(o.c) * most * most * most * most);
   return EGNN_OK;
 }
 

@@ -31,14 +31,21 @@ struct NsBatch {
   int count;
 };
 
-// X, A and B = b A + c A A are kept as fp16 pairs hi + lo (22 bits) scaled by
-// powers of two, chosen so that their largest entries stay near 2^14: the
-// iteration bounds the singular values, hence every entry, beforehand.
+// X, A and B = b A + c A A are kept as fp16 pairs hi + lo (22 bits), scaled by
+// powers of two of their own in every step, a factor 4 below fp16's largest value.
+// With the singular values, hence the entries, of X up to 2^e: X by 2^(14 - e),
+// A by 2^(14 - 2e), B by 2^(14 - eb) with 2^eb above |b| 2^2e + |c| 2^4e.  e starts
+// from |G| / (|G| + eps) and goes by the polynomial's bounds; one bound of all
+// steps would leave the early ones, or a gradient below eps, to fp16's smallest numbers
+// (coefficients 6, -3, 0.3 in two steps of 1024 x 4096: error 8.4e-6, so 1.4e-7;
+// |G| = 1e-14, eps = 1e-7: 2e-3, so 1.3e-7).
 struct NsScalars {
   float a, b, c;
   double eps;
-  float sx, sa, sb;         // scales of X, A and b A + c A A
-  float mu, nu;             // nu = 1 - mu
+  int8_t bound[kNsMaxSteps + 1];   // before step k the singular values are below 2^bound[k]
+  int8_t growth[kNsMaxSteps];      // and grow by at most 2^growth[k] in it
+  int a_exp, b_exp, c_exp;         // |a| <= 2^a_exp, ...
+  float mu, nu;                    // nu = 1 - mu
   double decay, lr;
   const float* lr_device;
   int nesterov;
@@ -68,6 +75,30 @@ __device__ __forceinline__ void ns_rates(const NsItem& it, const NsScalars& q, f
   keep = (float)(1.0 - lr * q.decay);
   move = (float)(-lr * it.gain);
 }
+
+// Smaller singular values than 2^kNsLeast are held with fewer bits.
+constexpr int kNsLeast = -56, kNsMostExp = 64;
+// 2^e; what is below float32's normal range is 0.
+__device__ __forceinline__ float ns_pow2(int e) { return e < -126 ? 0.f : __int_as_float((min(e, 127) + 127) << 23); }
+// The weights of a step whose X is below 2^e, of the scaled terms, and e for the next step.
+struct NsStep {
+  float b, cc;     // B = b A + cc (A A)
+  float x, bx;     // X' = x X + bx (B X), scaled for the next step, or X' itself after the last
+  __device__ NsStep() {}
+  __device__ __forceinline__ NsStep(const NsScalars& q, int step, int& e) {
+    const int eb = max(q.b_exp + 2 * e, q.c_exp + 4 * e) + 1;
+    // the polynomial's factor of s: its most over the step's whole range, or at 2^e and below
+    const int grown = e + min((int)q.growth[step], max(q.a_exp, eb - 1) + 2);
+    // 2^14: X' itself, not scaled
+    const int next = step + 1 < q.steps ? max(kNsLeast, min((int)q.bound[step + 1], grown)) : 14;
+    b = q.b * ns_pow2(2 * e - eb);
+    cc = q.c * ns_pow2(4 * e - eb - 14);
+    x = q.a * ns_pow2(e - next);
+    bx = ns_pow2(eb + e - next - 14);
+    e = next;
+  }
+};
+constexpr float kNsGram = 0x1p-14f;   // X X^T of scaled X -> scaled A, in every step
 
 // A sum in tensor memory is rounded towards zero at each of its L instructions.
 // On average one loses half a unit in the last place of the sum so far, which

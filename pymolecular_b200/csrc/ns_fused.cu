@@ -327,7 +327,9 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) ss += red[k];
     float pre, f;
-    norm_scale(ss, q.eps, pre, f);
+    int e;   // X is below 2^e
+    norm_scale(ss, q.eps, pre, f, e);
+    const float sx = ns_pow2(14 - e);
     // warp w owns tile rows 32 (w % 4) .. + 31, which are its accumulator lanes,
     // and of each group of four 32-column pieces the (w / 4)-th
     const int row = (warp & 3) * 32 + lane, piece = warp >> 2;
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
             store_raw16(hi, lo, h, v + 16 * h);
           } else {
 #pragma unroll
-            for (int j = 16 * h; j < 16 * h + 16; ++j) v[j] *= q.sx;
+            for (int j = 16 * h; j < 16 * h + 16; ++j) v[j] *= sx;
             store_pairs16(hi, lo, h, v + 16 * h);
           }
         }
@@ -359,14 +361,12 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
       }
     }
 
-    const float fA = q.sa / (q.sx * q.sx);                    // accumulator -> A scaled
-    const float fbA = q.b * q.sb / q.sa, fcAA = q.c * q.sb / (q.sa * q.sa);
-    const float fX = 1.f / q.sb, back = 1.f / q.sx;
     const float loss_n = ns_mean_loss((n16 >> 4) / sums), loss_m = ns_mean_loss(m16 >> 4);
     const bool a_here = rows_here && piece * 32 < m16;
     bool ok = true;
 #pragma unroll 1
     for (int step = 0; step < q.steps && ok; ++step) {
+      const NsStep w(q, step, e);
       // What does not wait for a product is fetched before the wait.  An accumulator is read
       // to its end before the first half is handed over, where the products of that half
       // write to its place.
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
           for (int k = 0; k < 16; ++k) t[k] += u[k];
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[16 * h + k] = (fmaf(t[k], loss_n, t[k]) + x[k]) * fA;
+        for (int k = 0; k < 16; ++k) v[16 * h + k] = (fmaf(t[k], loss_n, t[k]) + x[k]) * kNsGram;
       };
       if (!(ok = wait_bar(&bar.a_done, step, gave_up, q.wait_polls))) break;
       if (a_here) {
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
         arrive(&bar.a_ready[h]);
       }
 #pragma unroll
-      for (int k = 0; k < 32; ++k) v[k] *= fbA;
+      for (int k = 0; k < 32; ++k) v[k] *= w.b;
       if (!(ok = wait_bar(&bar.aa_done, step, gave_up))) break;
       if (a_here) {
 #pragma unroll
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
           tmem_ld16x2(tAA + c, tAAx + c, t, x);
 #pragma unroll
           for (int k = 0; k < 16; ++k)
-            v[16 * h + k] = fmaf(fcAA, x[k], fmaf(fcAA, fmaf(t[k], loss_m, t[k]), v[16 * h + k]));
+            v[16 * h + k] = fmaf(w.cc, x[k], fmaf(w.cc, fmaf(t[k], loss_m, t[k]), v[16 * h + k]));
         }
       }
 #pragma unroll
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
         if (here) {   // this thread's own
           load_pairs32(hi, lo, v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= q.a;
+          for (int j = 0; j < 32; ++j) v[j] *= w.x;
         }
         if (!(ok = wait_bar(&bar.slot_done[slot], slot_use(step, k), gave_up))) break;
         if (here) {
@@ -440,20 +440,15 @@ __global__ void __launch_bounds__(kThreads + 32, 1) ns_fused_kernel(const __grid
           tmem_ld16x2(c, c + 16, t, u);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            v[j] = fmaf(fX, fmaf(t[j], loss_m, t[j]), v[j]);
-            v[16 + j] = fmaf(fX, fmaf(u[j], loss_m, u[j]), v[16 + j]);
+            v[j] = fmaf(w.bx, fmaf(t[j], loss_m, t[j]), v[j]);
+            v[16 + j] = fmaf(w.bx, fmaf(u[j], loss_m, u[j]), v[16 + j]);
           }
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (here) {
-            if (step + 1 < q.steps) {
-              store_pairs16(hi, lo, h, v + 16 * h);
-            } else {
-#pragma unroll
-              for (int j = 16 * h; j < 16 * h + 16; ++j) v[j] *= back;
-              store_raw16(hi, lo, h, v + 16 * h);
-            }
+            if (step + 1 < q.steps) store_pairs16(hi, lo, h, v + 16 * h);
+            else store_raw16(hi, lo, h, v + 16 * h);
           }
           arrive(&bar.x_ready[k][h]);
         }

@@ -55,6 +55,7 @@ struct Work {
   char* x[2];            // images: hi blocks, then lo blocks
   char *a, *b;
   unsigned* counter;     // arrivals of the group's blocks, for each phase
+  int* start;            // X0 is below 2^start
   float* part;           // pieces of A
   double* partial;       // sums of squares of the parts of U
 };
@@ -174,7 +175,10 @@ __global__ void __launch_bounds__(256) ns_image_kernel(const __grid_constant__ G
   double ss = 0.0;
   for (int k = 0; k < kParts; ++k) ss += g.w[blockIdx.y].partial[k];
   float pre, f;
-  norm_scale(ss, q.eps, pre, f);
+  int e;
+  norm_scale(ss, q.eps, pre, f, e);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *g.w[blockIdx.y].start = e;
+  const float sx = ns_pow2(14 - e);
   char* const hi = g.w[blockIdx.y].x[0];
   char* const lo = hi + sh.x_bytes();
   const int rows = sh.turn ? sh.xc * 64 : sh.bands * 128, cols = sh.turn ? sh.bands * 128 : sh.xc * 64;
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(256) ns_image_kernel(const __grid_constant__ G
     const size_t band = to_band(t, sh.xc, sh.turn);
     if (q.steps) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] *= q.sx;
+      for (int k = 0; k < 8; ++k) v[k] *= sx;
       unit_to_pairs(hi + band, lo + band, 128, sh.turn, t, v);
     } else {
       unit_to_raw(hi + band, lo + band, kBlk, sh.turn, t, v);
@@ -343,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   __shared__ Barriers bar;
   __shared__ uint32_t tmem_s;
   __shared__ Phase phase[4];
+  __shared__ NsStep weights[kNsMaxSteps];
   __shared__ int gave_up_s;
   const int lane = threadIdx.x & 31;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -356,6 +361,13 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   volatile int* const gave_up = &gave_up_s;
 
   if (warp == 0 && lane < sh.per_step()) phase[lane].set(sh, lane);
+  if (warp == 2) {
+    int e = *w.start;
+    for (int k = 0; k < q.steps; ++k) {
+      const NsStep s(q, k, e);
+      if (lane == 0) weights[k] = s;
+    }
+  }
   if (warp == 1) {
     tmem_alloc(&tmem_s, 512);
     if (lane == 0) {
@@ -512,6 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const float loss = ns_mean_loss(4 * segment);
     int seg = 0, outs = 0, sent = 0;
+    const NsStep* step = weights;
     // The readers' arrival at `written`.  A warp arrives again only when the last round is
     // complete: arrivals are counted, not the warps, and a fast one's second would stand for a slow
     // one's first.
@@ -525,7 +538,11 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
     uint32_t parity = 0;   // of each stage's next filling
 #pragma unroll 1
     for (int p = 0, phase_of_step = 0, cur = 0; p < phases && ok; ++p, ++phase_of_step) {
-      if (phase_of_step == per_step) phase_of_step = 0, cur ^= 1;
+      if (phase_of_step == per_step) {
+        phase_of_step = 0;
+        cur ^= 1;
+        ++step;
+      }
       const Phase& f = phase[phase_of_step];
       const int mode = f.mode;
       if (mode == 3) {
@@ -542,9 +559,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
       char* const dst = mode == 0 ? w.a : mode == 1 ? w.b : w.x[cur ^ 1];
       const bool last = p + 1 == phases;   // X' itself, not scaled
       // weights of the product and of the old tile
-      const float end = last ? 1.f / q.sx : 1.f;
-      const float wp = mode == 0 ? q.sa / (q.sx * q.sx) : mode == 1 ? q.c * q.sb / (q.sa * q.sa) : end / q.sb;
-      const float wo = mode == 1 ? q.b * q.sb / q.sa : q.a * end;
+      const float wp = mode == 0 ? kNsGram : mode == 1 ? step->cc : step->bx;
+      const float wo = mode == 1 ? step->b : step->x;
 #pragma unroll 1
       for (int t = rank; mode != 3 && t < f.tiles && ok; t += group) {
         const Tile at(f, t);
@@ -691,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
       if (warp == 2 && lane == 0) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         fence_proxy_async_all();
-        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(w.counter + p) : "memory");
+        if (!last) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(w.counter + p) : "memory");
       }
       __syncwarp();
     }
@@ -765,7 +781,8 @@ Work carve_work(Carver& c, const Shape& s) {
   w.a = c.take<char>(2 * s.a_bytes());
   w.b = c.take<char>(2 * s.a_bytes());
   w.partial = c.take<double>(kParts);
-  w.counter = c.take<unsigned>(4 * kNsMaxSteps);
+  w.counter = c.take<unsigned>(4 * kNsMaxSteps);   // the last of 4 kNsMaxSteps phases has none
+  w.start = reinterpret_cast<int*>(w.counter + 4 * kNsMaxSteps - 1);
   w.part = c.take<float>(s.part_bytes() / 4);
   return w;
 }

@@ -209,8 +209,9 @@ __device__ __forceinline__ float scaled_down(double x, int e) {
 // 1 / (sqrt(ss) + eps) as pre * f, so that both are float32 at any norm: norm and
 // eps are brought near 1 by the power of two h of the larger, and half of it goes
 // to each factor.  Float32 arithmetic: a float64 square root and division took
-// 3,000 cycles of a block's time.
-__device__ __forceinline__ void norm_scale(double ss, double eps, float& pre, float& f) {
+// 3,000 cycles of a block's time.  bound: the norm after it is at most 2^bound.
+__device__ __forceinline__ void norm_scale(double ss, double eps, float& pre, float& f, int& bound) {
+  bound = 0;
   const int e = ((__double2hiint(ss) >> 20) & 0x7ff) - 1023;   // -1023: zero; 1024: infinity or NaN
   if (e == 1024) {
     pre = 1.f;
@@ -225,6 +226,7 @@ __device__ __forceinline__ void norm_scale(double ss, double eps, float& pre, fl
   const int h1 = h / 2;
   pre = ldexpf(1.f, -h1);
   f = ldexpf(t, h1 - h);
+  bound = max(kNsLeast, min(0, (__float_as_int(norm * t) >> 23 & 255) - 126));
 }
 
 // ---- waits -------------------------------------------------------------------

@@ -1,10 +1,12 @@
 """Calls of the layer norm, the orthogonalisation and the momentum step that
 have to be refused, or answered without a launch, shown without a GPU."""
+import ctypes as C
+
 import pytest
 import torch
 from torch import nn
 
-from pymolecular_b200 import layer_norm, muon_step, orthogonalize
+from pymolecular_b200 import _native as nat, layer_norm, muon_step, orthogonalize
 
 
 class OnDevice(torch.Tensor):
@@ -42,3 +44,21 @@ def test_tracing_of_results_written_by_pointer_is_refused():
     for call in (orthogonalize, lambda w: orthogonalize([w, w])[0], step):
         with pytest.raises(RuntimeError, match="trace"):
             torch.jit.trace(lambda t: call(t.as_subclass(OnDevice)), (torch.ones(4, 4),))
+
+
+@pytest.mark.parametrize("steps,coefficients,taken", [
+    (2, (0.0, 3.0, -1.0), False),     # s^3: 2 for s = 1, 6e-4 for s = 0.06
+    (1, (0.0, 3.0, -1.0), True),      # nothing is held between steps
+    (2, (0.125, 1.0, 1.0), False),    # 2.125 against 1/8 s: 17 times
+    (2, (0.125, 1.0, 0.5), True),     # 13 times
+    (6, (0.5, 0.5, 0.0), False),      # 1 against 2^-5 before the last step
+    (5, (0.5, 0.5, 0.0), True),       # 16 times
+    (64, (1.875, -1.25, 0.375), True)])
+def test_coefficients_that_leave_small_singular_values_behind(steps, coefficients, taken):
+    """The operands' scales follow the largest singular value that the
+    coefficients allow; beside it small ones have to keep their bits."""
+    o = nat.NsOptions(steps, 0, *coefficients, 1e-7)
+    m = nat.Matrix(16, 16, 8, 8, 4, 8, nat.DTYPE_F32, 0)
+    status = nat.lib().egnn_orthogonalize(1, (nat.Matrix * 1)(m), C.byref(o), None, 0, None)   # no workspace: no launch
+    assert status == (nat.EGNN_ERR_WORKSPACE if taken else nat.EGNN_ERR_INVALID_ARG)
+    assert taken or "fall too far behind" in nat.last_error()
