@@ -404,7 +404,8 @@ typedef struct {
 /* For every matrix: momentum <- mu momentum + (1 - mu) grad;
  * U = mu momentum + (1 - mu) grad (nesterov) or momentum;
  * weight <- (1 - lr weight_decay) weight - lr gain orthogonalised(U).
- * Weights and momenta are updated in place; deterministic. */
+ * Weights and momenta are updated in place; deterministic.  Where a wait ran
+ * out (egnn_device_status) the weight stays as it was. */
 EGNN_API int egnn_muon_step(int64_t count, const egnn_muon_matrix* m, const egnn_muon_options* o, void* workspace,
                             size_t workspace_bytes, void* stream);
 

@@ -55,10 +55,11 @@ struct Work {
   char* x[2];            // images: hi blocks, then lo blocks
   char *a, *b;
   unsigned* counter;     // arrivals of the group's blocks, for each phase
-  int* start;            // X0 is below 2^start
+  int* start;            // X0 is below 2^start; kGaveUp: a wait ran out, the image is not complete
   float* part;           // pieces of A
   double* partial;       // sums of squares of the parts of U
 };
+constexpr int kGaveUp = 1 << 20;
 constexpr int kItems = kNsLarge;   // matrices of one launch
 struct Grid {
   NsItem it[kItems];
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(256) ns_image_kernel(const __grid_constant__ G
 }
 
 // ---- the result out of the image, or the weight moved by it --------------------
+// A matrix whose iteration gave up is left alone: there are no numbers in its image.
 template <typename T>
 __device__ __forceinline__ void give(const NsItem& it, const NsScalars& q, const Shape& sh, const char* hi, const char* lo) {
   T* const out = static_cast<T*>(it.out);
@@ -229,6 +231,7 @@ __device__ __forceinline__ void give(const NsItem& it, const NsScalars& q, const
 __global__ void __launch_bounds__(256) ns_give_kernel(const __grid_constant__ Grid g, const __grid_constant__ NsScalars q) {
   pdl_enter();
   const NsItem& it = g.it[blockIdx.y];
+  if (*g.w[blockIdx.y].start == kGaveUp) return;
   const Shape sh(it);
   const char* hi = g.w[blockIdx.y].x[q.steps & 1];
   const char* lo = hi + sh.x_bytes();
@@ -717,7 +720,10 @@ __global__ void __launch_bounds__(kThreads, 1) ns_grid_kernel(const __grid_const
   fence_before_sync();
   __syncthreads();
   if (warp == 1) {
-    if (lane == 0 && *gave_up) atomicAdd(&g_ns_grid_timeouts, 1);
+    if (lane == 0 && *gave_up) {
+      *w.start = kGaveUp;
+      atomicAdd(&g_ns_grid_timeouts, 1);
+    }
     tmem_dealloc(tmem, 512);
   }
 }

@@ -5,7 +5,7 @@ import torch
 from torch import nn
 from torch.autograd import forward_ad
 
-from pymolecular_b200 import layer_norm, orthogonalize
+from pymolecular_b200 import _native as nat, layer_norm, muon_step, orthogonalize
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,30 @@ def test_matrices_with_an_empty_side(shape, cuda_device):
     for dtype in (torch.float32, torch.bfloat16):
         out = orthogonalize(torch.zeros(shape, dtype=dtype, device=cuda_device))
         assert out.shape == shape and out.dtype == dtype and out.device == cuda_device
+
+
+@pytest.mark.parametrize("shapes", [[(64, 129), (128, 257)], [(200, 333), (256, 513)], [(64, 2000), (40, 50)],
+                                    [(256, 513)] * 30])
+def test_a_step_whose_waits_run_out_leaves_the_weights(shapes, cuda_device, monkeypatch):
+    """EGNN_DEBUG_WAIT_POLLS=0: the readers of either kernel give up at once
+    (the products complete and are drained).  There is no update then, and
+    none is made of what lies in the workspace."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    w0, grads, m0 = ([torch.randn(*s, device=cuda_device, generator=g) for s in shapes] for _ in range(3))
+    lib = nat.lib()
+
+    def step():
+        w, m = [t.clone() for t in w0], [t.clone() for t in m0]
+        muon_step(w, grads, m, lr=0.1, weight_decay=0.1)
+        return w, m
+
+    monkeypatch.delenv("EGNN_DEBUG_WAIT_POLLS", raising=False)
+    want = step()
+    assert lib.egnn_device_status(nat.stream_ptr()) == nat.EGNN_OK, nat.last_error()
+    monkeypatch.setenv("EGNN_DEBUG_WAIT_POLLS", "0")
+    w, m = step()
+    assert lib.egnn_device_status(nat.stream_ptr()) == nat.EGNN_ERR_CUDA and "timed out" in nat.last_error()
+    assert all(torch.equal(a, b) for a, b in zip(w, w0))
+    assert all(torch.equal(a, b) for a, b in zip(m, want[1]))
+    monkeypatch.delenv("EGNN_DEBUG_WAIT_POLLS")
+    assert all(torch.equal(a, b) for a, b in zip(sum(step(), []), sum(want, [])))
