@@ -31,6 +31,9 @@ from .norm import DTYPES
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 STEPS = 5
 EPS = 1e-7
+MAX_SIDE, MAX_SMALL_SIDE = 16384, 1024
+TOO_LARGE = f"matrices have at most {MAX_SIDE} rows and columns, and the smaller side at most {MAX_SMALL_SIDE}"
+NOT_DENSE = "parameters and momenta must have dense rows (they are updated in place)"
 
 
 @functools.lru_cache(maxsize=64)
@@ -44,8 +47,13 @@ def _workspace(sizes: Sequence[int], device) -> Tuple[torch.Tensor, int]:
     if max(sizes) < 1 << 31:
         nbytes = nat.lib().egnn_orthogonalize_workspace_size(len(sizes) // 2, struct.pack("%di" % len(sizes), *sizes))
     if not nbytes:
-        raise ValueError("matrices have at most 16384 rows and columns, and the smaller side at most 1024")
+        raise ValueError(TOO_LARGE)
     return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+
+
+def _dense_rows(t: torch.Tensor) -> bool:
+    rows, cols = t.shape
+    return not rows * cols or (t.stride(1) == 1 or cols <= 1) and (t.stride(0) >= cols or rows <= 1)
 
 
 def _refuse_tracing(t: torch.Tensor) -> None:
@@ -161,9 +169,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
         ldp = ldg = ldm = cols
         if not (p.is_contiguous() and m.is_contiguous()):
             ldp, ldm = p.stride(0), m.stride(0)
-            for t, ld in ((p, ldp), (m, ldm)):
-                if rows * cols and (t.stride(1) != 1 and cols > 1 or ld < cols and rows > 1):
-                    raise ValueError("parameters and momenta must have dense rows (they are updated in place)")
+            if not (_dense_rows(p) and _dense_rows(m)):
+                raise ValueError(NOT_DENSE)
         if not g.is_contiguous():
             if g.stride(1) == 1 and g.stride(0) >= cols:
                 ldg = g.stride(0)
@@ -195,7 +202,8 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], buf
 class Muon(torch.optim.Optimizer):
     """Momentum with orthogonalised updates for weight matrices.
 
-    Takes float32 matrices only: an ``EGNN``'s weights go here, its biases and
+    Takes float32 matrices with dense rows and of the sizes that
+    ``muon_step`` takes: an ``EGNN``'s weights go here, its biases and
     normalisation vectors to another optimiser (``Muon.split``).  `lr` may be
     a one-element CUDA tensor (captured steps).  State: ``momentum_buffer``.
     """
@@ -215,10 +223,17 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
         for p in self.param_groups[-1]["params"]:
+            wrong = None   # with what a step would refuse, before a backward has been paid for
             if p.dim() != 2 or p.dtype != torch.float32:
+                wrong = (f"Muon takes float32 matrices, got {tuple(p.shape)} {p.dtype} (Muon.split gives them and "
+                         "the rest apart)")
+            elif max(p.shape) > MAX_SIDE or min(p.shape) > MAX_SMALL_SIDE:
+                wrong = f"{TOO_LARGE}, got {tuple(p.shape)}"
+            elif not _dense_rows(p):
+                wrong = f"{NOT_DENSE}, got {tuple(p.shape)} with strides {p.stride()}"
+            if wrong:
                 del self.param_groups[-1]
-                raise ValueError(f"Muon takes float32 matrices, got {tuple(p.shape)} {p.dtype} (Muon.split gives them and "
-                                 "the rest apart)")
+                raise ValueError(wrong)
 
     @staticmethod
     def split(params: Iterable[torch.Tensor]) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:

@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch import nn
 
-from pymolecular_b200 import _native as nat, layer_norm, muon_step, orthogonalize
+from pymolecular_b200 import Muon, _native as nat, layer_norm, muon_step, orthogonalize
 
 
 class OnDevice(torch.Tensor):
@@ -62,3 +62,23 @@ def test_coefficients_that_leave_small_singular_values_behind(steps, coefficient
     status = nat.lib().egnn_orthogonalize(1, (nat.Matrix * 1)(m), C.byref(o), None, 0, None)   # no workspace: no launch
     assert status == (nat.EGNN_ERR_WORKSPACE if taken else nat.EGNN_ERR_INVALID_ARG)
     assert taken or "fall too far behind" in nat.last_error()
+
+
+@pytest.mark.parametrize("make,match", [
+    (lambda: torch.zeros(1025, 1025), "at most"), (lambda: torch.zeros(2, 16385), "at most"),
+    (lambda: torch.zeros(16385, 1), "at most"), (lambda: torch.zeros(6, 4).t(), "dense rows"),
+    (lambda: torch.zeros(6, 8)[:, ::2], "dense rows"), (lambda: torch.zeros(1, 4).expand(6, 4), "dense rows")])
+def test_muon_refuses_matrices_that_no_step_can_take(make, match):
+    """When it is made, and not at the first step."""
+    good = nn.Parameter(torch.zeros(4, 6))
+    with pytest.raises(ValueError, match=match):
+        Muon([good, nn.Parameter(make())])
+    opt = Muon([good])
+    with pytest.raises(ValueError, match=match):
+        opt.add_param_group({"params": [nn.Parameter(make())]})
+    assert len(opt.param_groups) == 1
+
+
+def test_muon_takes_what_a_step_takes():
+    Muon([nn.Parameter(t) for t in (torch.zeros(1024, 2000), torch.zeros(16384, 1024), torch.zeros(3, 20)[:, 2:9],
+                                    torch.zeros(0, 5), torch.zeros(1, 5).t(), torch.zeros(6, 5)[:, :1])])
