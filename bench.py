@@ -46,6 +46,8 @@ def parse():
                          "faster at 2 and 8 GPUs) or per-layer buckets all-reduced as the backward "
                          "produces them (layers)")
     ap.add_argument("--no-e2e", action="store_true")
+    ap.add_argument("--details", metavar="FILE", help="write every figure of the run (kernel groups, the other workloads' "
+                                                      "records) to FILE as JSON; the printed line has the main ones")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-extras", action="store_true",
                     help="skip the fp32-mode and other-workload measurements of the default 1-GPU run")
@@ -658,6 +660,35 @@ def make_line(args, prob, m, world, clk, cpu, dev):
     }
 
 
+def rounded(v):
+    """Floats to six digits, through dicts and lists."""
+    if isinstance(v, dict):
+        return {k: rounded(x) for k, x in v.items()}
+    if isinstance(v, (list, tuple)):
+        return [rounded(x) for x in v]
+    return float(f"{v:.6g}") if isinstance(v, float) else v
+
+
+def printed(line):
+    """The one line that is printed: `line` without what only a reader of all
+    figures needs.  Readers that keep the last 3,000 characters of the output must get it
+    whole (with everything it was 20,000 long)."""
+    out = {k: v if k in ("value", "ms_per_step") else rounded(v) for k, v in line.items()}
+    if out.get("roofline"):
+        out["roofline"] = {k: v for k, v in out["roofline"].items()
+                           if k in ("kernel", "bound", "achieved", "peak", "unit", "frac", "per_launch_ms", "traffic")}
+        out["roofline"]["groups"] = {k: round(v["frac"], 4) for k, v in line["roofline"]["groups"].items()}
+    if out.get("e2e"):
+        out["e2e"] = {k: v for k, v in out["e2e"].items() if k != "eager"}
+        if "eager" in line["e2e"]:
+            out["e2e"]["eager_value"] = rounded(line["e2e"]["eager"]["value"])
+    if out.get("extras"):
+        out["extras"] = {k: {"ms_per_step": round(v["ms_per_step"], 4), "frac": rounded(v["roofline"].get("frac")),
+                             "device_status": v["device_status"]} for k, v in line["extras"].items()}
+    out.pop("kernel_ms_per_step", None)
+    return out
+
+
 def cpu_baseline(cfg_id, steps):
     threads = os.cpu_count() or 1
     sample = cpu_sample_size(cfg_id)
@@ -739,7 +770,9 @@ def run_b200(args):
             del p2
             torch.cuda.empty_cache()
     if rank == 0:
-        print(json.dumps(line), flush=True)
+        if args.details:
+            Path(args.details).write_text(json.dumps(line) + "\n")
+        print(json.dumps(printed(line)), flush=True)
     if world > 1:
         dist.barrier()
         dist.destroy_process_group()
