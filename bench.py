@@ -1,7 +1,7 @@
 #!/usr/bin/env python
 """EGNN training-step benchmark (layer fwd+bwd edges/s, molecules/s).
 
-    python bench.py [--gpus N] [--steps K] [--warmup W] [--config 2] [--impl b200|reference]
+    python bench.py [--gpus N] [--steps K] [--warmup W] [--config 2] [--impl b200|reference] [--details FILE]
 
 One step = forward of the whole EGNN over one batch of synthetic graphs,
 graph-sum MSE loss, backward, gradient all-reduce (N > 1) and an SGD update

@@ -137,7 +137,8 @@ int run_all(const char* what, int64_t count, const Fill& fill, const NsScalars& 
   const Carver c(ws);
   // A few small matrices among large ones (embeddings among wide layers) run beside
   // them, on SMs that the large ones leave: five of up to 128 x 31 with 200 x 333,
-  // 64 x 1100 and 513 x 97 take 171 us, one kernel after the other 191.
+  // 64 x 1100 and 513 x 97 take 120 us, one kernel after the other 139; 18 of 128 x 257
+  // with six H = 256 layers 190 and 241.
   struct Side {
     cudaStream_t main_s, stream;
     int status = EGNN_OK;

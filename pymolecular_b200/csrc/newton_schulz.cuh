@@ -12,7 +12,7 @@
 namespace egnn {
 
 // Matrices of one batch: as many as fill the device with one block each (10 KB of kernel
-// parameters; 140 of 128 x 257 take 60 us, in batches of 64 166 us).
+// parameters; 140 of 128 x 257 take 54 us, in batches of 64 158 us).
 constexpr int kNsItems = 160;
 constexpr int kNsLarge = 64;   // matrices of a batch that go through the workspace, which batches share
 constexpr int kNsMaxSteps = 64;

@@ -7,7 +7,8 @@
 // (2^-22 of the result) is left out.  Sums in tensor memory are rounded towards
 // zero at every instruction, by the size of the sum so far: lo hi + hi lo goes
 // into an accumulator of its own, or in before hi hi, so that only one
-// instruction per 16 terms costs a rounding of the full sum.
+// instruction per 16 terms costs a rounding of the full sum.  The hi hi terms of
+// X X^T are one sum up to n = 384 and three beyond, those of the other products one.
 //
 // X (hi, lo) and A, then B, (hi, lo) stay in shared memory through all steps:
 // global memory sees the matrix once on the way in and once on the way out.
@@ -19,7 +20,7 @@
 // 128 x 257 takes 14,000 cycles, its products alone 8,300 (three half-precision
 // products each), the rest are accumulators on their way through the registers.
 // 5 steps of one 64 x 129 take 30 us, of one 128 x 257 and of 35 of them 53 us, against
-// 71, 93 and 130 us in the kernel for large matrices, which takes 100 us for 128 x 321.  A matrix on a cluster of two blocks was slower (65 us for the 35, then 55 without): 64 KB
+// 77, 99 and 134 us in the kernel for large matrices, which takes 102 us for 128 x 321.  A matrix on a cluster of two blocks was slower (65 us for the 35, then 55 without): 64 KB
 // through distributed shared memory cost 9,000 cycles a step.
 #include <atomic>
 

@@ -21,9 +21,9 @@
 //
 // What bounds it: the chain of a product, some 13,000 cycles of which the tensor cores
 // work 2,000 to 7,000: meeting and first copies 3,400, the last accumulator's way into
-// shared memory 2,800, from there into L2 3,500.  One 200 x 333 takes 106 us for 5 steps,
-// the 30 matrices of six H = 256 layers 180 us: 13 GF, three times in half precision, is 24 us
-// of the measured matrix rate.
+// shared memory 2,800, from there into L2 3,500.  One 200 x 333 takes 114 us for 5 steps,
+// the 30 matrices of six H = 256 layers 187 us, 30 of 256 x 513 201 us: the six layers' 13 GF,
+// three times in half precision, are 24 us of the measured matrix rate.
 //
 // Sums in tensor memory are rounded towards zero at every instruction, by the
 // size of the sum so far.  So lo hi + hi lo has an accumulator of its own, and
@@ -72,10 +72,10 @@ constexpr int kParts = 32;   // blocks of a matrix in the norm
 // A's sum runs over the long side.  It is split into pieces of at least kSplit chunks
 // of 64 columns, which a group's blocks compute side by side, as float32, and add up,
 // in order, in a phase of its own.  The pieces' number follows from the matrix alone,
-// and with it the result.  In pieces and whole: 64 x 1100 110 and 137 us, 128 x 900 125
-// and 135, 1 x 16384 158 and 848.  From 9 chunks on it is no gain where bands fill the
-// device: 1024 x 1024 305 and 245; pieces of 4 make 30 matrices of 256 x 513 slower
-// (242 and 194), of 9 leave 64 x 1100 at 131.
+// and with it the result.  In pieces and whole: 64 x 1100 107 and 135 us, 128 x 900 130
+// and 141, 1 x 16384 164 and 861.  It is no gain where bands fill the device: 1024 x 1024
+// 280 and 238; pieces of 4 make 30 matrices of 256 x 513 slower (238 and 201), of 9 leave
+// 64 x 1100 at 119.
 constexpr int kSplit = 6, kMostPieces = 64;   // of them all tiles
 
 struct Shape {
@@ -770,8 +770,8 @@ int allot(const Grid& g, int blocks, int tile, int* size) {
 }
 
 // Tiles 64 or 128 columns wide, whichever let the longest step end first: 64 make more
-// of them, each sooner done.  64 and 128: 200 x 333 110 and 130 us, 16 matrices of 256 x 513
-// 153 and 180, 30 of them 208 and 179.
+// of them, each sooner done.  64 and 128: 200 x 333 114 and 134 us, 16 matrices of 256 x 513
+// 151 and 182, 30 of them 239 and 201, six H = 256 layers 213 and 187.
 void share_out(Grid& g, int blocks) {
   int size64[kItems], size128[kItems];
   g.tile = allot(g, blocks, 64, size64) < allot(g, blocks, 128, size128) ? 64 : 128;

@@ -69,19 +69,14 @@ __device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint6
       : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate));
 }
 
-// kind::f16 takes both 16-bit types; the instruction descriptor says which.
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                        uint32_t accumulate) {
-  mma_bf16(d_tmem, a_desc, b_desc, idesc, accumulate);
-}
-
 // One lane of a converged warp (1 there, 0 in the others).
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t e;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
   return e;
 }
-// mma_f16 by the elected lane of a warp that is here as a whole: the loop
+// The same product (kind::f16 takes both 16-bit types; the instruction descriptor says
+// which) by the elected lane of a warp that is here as a whole: the loop
 // around it is uniform over the warp, so that descriptors stay in uniform
 // registers (measured: 85 cycles an instruction when one thread loops alone).
 __device__ __forceinline__ void mma_f16_elected(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
