@@ -76,10 +76,13 @@ __device__ __forceinline__ void ns_rates(const NsItem& it, const NsScalars& q, f
   move = (float)(-lr * it.gain);
 }
 
-// Smaller singular values than 2^kNsLeast are held with fewer bits.
-constexpr int kNsLeast = -56, kNsMostExp = 64;
-// 2^e; what is below float32's normal range is 0.
-__device__ __forceinline__ float ns_pow2(int e) { return e < -126 ? 0.f : __int_as_float((min(e, 127) + 127) << 23); }
+// Smaller singular values than 2^kNsLeast are held with fewer bits: 2^(14 - kNsLeast) is a
+// float32, and |G| / (|G| + 1e-7) is above it for any float32 |G| above the smallest normal one.
+constexpr int kNsLeast = -112, kNsMostExp = 64;
+// 2^e; 0 below float32's range.
+__device__ __forceinline__ float ns_pow2(int e) {
+  return e < -149 ? 0.f : __int_as_float(e < -126 ? 1 << (e + 149) : (min(e, 127) + 127) << 23);
+}
 // The weights of a step whose X is below 2^e, of the scaled terms, and e for the next step.
 struct NsStep {
   float b, cc;     // B = b A + cc (A A)

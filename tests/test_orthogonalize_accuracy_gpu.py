@@ -67,10 +67,10 @@ def test_coefficients(rows, cols, steps, coefficients, cuda_device):
     assert own <= FACTOR * plain, (own, plain)
 
 
-@pytest.mark.parametrize("norm", [1e-8, 1e-12, 1e-16, 1e-20, 1e-23])
+@pytest.mark.parametrize("norm", [1e-8, 1e-12, 1e-16, 1e-20, 1e-23, 1e-28, 1e-33])
 @pytest.mark.parametrize("rows,cols", [(64, 129), (256, 513)])
 def test_gradients_far_below_eps(rows, cols, norm, cuda_device):
-    """The result shrinks with the gradient, and keeps its bits: |G| / (|G| + eps) down to 2^-53."""
+    """The result shrinks with the gradient, and keeps its bits: |G| / (|G| + eps) down to 2^-86."""
     g = torch.Generator(device="cuda").manual_seed(1)
     G = _gradient(rows, cols, g)
     G = G * (norm / G.norm())
@@ -80,6 +80,15 @@ def test_gradients_far_below_eps(rows, cols, norm, cuda_device):
         w, m = torch.zeros_like(G), torch.zeros_like(G)
         muon_step([w], [G], [m], lr=1.0, momentum=0.0)
         assert ((w + orthogonalize(G) * max(1, rows / cols) ** 0.5).norm() / w.norm()).item() <= 4 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 129), (256, 513)])
+def test_a_cubic_step_far_below_eps(rows, cols, cuda_device):
+    """Without a linear term nothing else covers what such a gradient's cube comes to."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    G = _gradient(rows, cols, g)
+    own, plain = _errors(G * (1e-18 / G.norm()), steps=1, coefficients=(0.0, 3.0, -1.0))
+    assert own <= FACTOR * plain, (own, plain)
 
 
 def test_small_singular_values(cuda_device):
