@@ -373,9 +373,11 @@ EGNN_API size_t egnn_orthogonalize_workspace_size(int64_t count, const int32_t* 
 /* out_k = the orthogonalised in_k for every matrix of the HOST array `m`
  * (read before the call returns).  The products' operands have 22 bits,
  * their sums float32's 24: against float64 the result of the usual five steps
- * is off by 1e-6 to 4e-6 in the 2-norm.  That is 0.3 to 1.9 times what the same
- * iteration in float32 is off by where both sides are 16 or more, and several
- * times that (as 22 bits are to 24) where one is smaller.  Deterministic.  No counterpart in the reference. */
+ * is off by 1e-6 to 4e-6 in the 2-norm for random matrices, by up to 5e-5 for
+ * a model's gradients, whose singular values fall off steeply.  That is 0.3 to
+ * 1.9 times what the same iteration in float32 is off by where both sides are 16
+ * or more, and several times that (as 22 bits are to 24) where one is smaller.
+ * Deterministic.  No counterpart in the reference. */
 EGNN_API int egnn_orthogonalize(int64_t count, const egnn_matrix* m, const egnn_ns_options* o, void* workspace,
                                 size_t workspace_bytes, void* stream);
 

@@ -22,7 +22,7 @@
 // What bounds it: the chain of a product, some 13,000 cycles of which the tensor cores
 // work 2,000 to 7,000: meeting and first copies 3,400, the last accumulator's way into
 // shared memory 2,800, from there into L2 3,500.  One 200 x 333 takes 114 us for 5 steps,
-// the 30 matrices of six H = 256 layers 187 us, 30 of 256 x 513 201 us: the six layers' 13 GF,
+// the 30 matrices of six H = 256 layers 187 us, 30 of 256 x 513 201 to 212 us: the six layers' 13 GF,
 // three times in half precision, are 24 us of the measured matrix rate.
 //
 // Sums in tensor memory are rounded towards zero at every instruction, by the
